@@ -230,6 +230,78 @@ VCB_API size_t vcb_forward_workspace(const vcb_forward_args* args);
  * scale, k_smooth, hadamard) (bindings.cpp:100-178) */
 VCB_API int vcb_forward(const vcb_forward_args* args, void* stream);
 
+/* ---- around the attention: projections, Q/K norm and rotation ------------------
+ * These entry points have no reference counterpart: the reference receives
+ * post-RoPE Q/K/V from the model (core.py:243-262).  Tensors are addressed by
+ * strides in elements; the last axis is contiguous.  Non-finite values pass
+ * through by IEEE rules.  Added without a change of the structures above, so
+ * the ABI version stays. */
+enum vcb_activation {
+    VCB_ACT_NONE = 0,
+    VCB_ACT_SILU = 1,
+    VCB_ACT_GELU = 2,               /* 0.5 y (1 + erf(y / sqrt 2)) */
+    VCB_ACT_GELU_TANH = 3,          /* 0.5 y (1 + tanh(sqrt(2/pi) (y + 0.044715 y^3))) */
+    VCB_ACT_RELU = 4
+};
+
+/* y[b, s, n] = residual[b, s, n] + gate[b, s, n] * act(sum_k x[b, s, k] w[n, k] + bias[n]),
+ * summed in FP32 and rounded once.  k runs over heads_in x k_head channels:
+ * element (b, h, s, c) of x is x[b * x_stride_b + h * x_stride_h + s * x_stride_s + c]
+ * (heads_in = 1: token-major x).  Column n of y is channel n % n_head of head
+ * n / n_head (n_head = n: token-major y). */
+typedef struct {
+    const void* x;
+    const void* w;                  /* [n, heads_in * k_head], rows w_stride apart */
+    int dtype;                      /* of x, w, residual and y: VCB_F16 or VCB_BF16 */
+    int64_t batch, tokens, n;
+    int64_t heads_in, k_head;
+    int64_t x_stride_b, x_stride_h, x_stride_s, w_stride;
+    const void* bias;               /* [n] or NULL */
+    int bias_dtype;                 /* vcb_dtype */
+    int activation;                 /* vcb_activation */
+    const void* gate;               /* or NULL; strides of 0 broadcast */
+    int gate_dtype;                 /* vcb_dtype */
+    int64_t gate_stride_b, gate_stride_s;
+    const void* residual;           /* or NULL; may be y itself */
+    int64_t residual_stride_b, residual_stride_s;
+    void* y;
+    int64_t n_head;                 /* divides n */
+    int64_t y_stride_b, y_stride_h, y_stride_s;
+    int32_t* status;                /* device status word (nullable); flags are ORed in */
+    void* workspace;
+    size_t workspace_bytes;
+} vcb_linear_args;
+
+/* bytes of scratch the call needs (may be 0); 0 for sizes the call would refuse */
+VCB_API size_t vcb_linear_workspace(const vcb_linear_args* args);
+VCB_API int vcb_linear(const vcb_linear_args* args, void* stream);
+
+/* Per head row x of Q and of K: n = x * weight / sqrt(mean(x^2) + eps) (norm;
+ * else n = x * weight), then (a, b) -> (a cos - b sin, a sin + b cos) for the
+ * rotary / 2 pairs: channels (2i, 2i + 1) when interleaved, (i, i + rotary / 2)
+ * otherwise.  Tokens at or behind `rows` are not rotated.  An output may be
+ * its own input. */
+typedef struct {
+    const void* q; const void* k;
+    void* q_out; void* k_out;
+    int dtype;                      /* vcb_dtype of q, k and the outputs */
+    int64_t batch, q_heads, k_heads, tokens;
+    int d;                          /* 1..128 */
+    int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3];   /* batch, head, token */
+    const void* q_weight;           /* [d] or NULL */
+    const void* k_weight;
+    int weight_dtype;               /* vcb_dtype of both */
+    const float* cos;               /* [batch or 1][rows][rotary / 2] */
+    const float* sin;
+    int64_t rows;                   /* 0..tokens */
+    int rotary;                     /* even, 0..d */
+    int64_t table_stride_b, table_stride_s;
+    int interleaved, norm;
+    float eps;
+} vcb_qk_norm_rope_args;
+
+VCB_API int vcb_qk_norm_rope(const vcb_qk_norm_rope_args* args, void* stream);
+
 /* Reads the device status word into *flags: one device-to-host copy ordered
  * on `stream` (not on the legacy default stream), then a wait for `stream`
  * only.  The one call of this library that blocks the host. */

@@ -1,0 +1,138 @@
+"""Arguments that the layer operators refuse, before they touch a device."""
+import ctypes
+
+import pytest
+import torch
+
+from vc_attention_b200 import _abi, linear, qk_norm_rope
+from vc_attention_b200.layer import _overlaps_itself, _shares_memory
+
+BF16 = torch.bfloat16
+
+
+def _t(*shape, dtype=BF16):
+    return torch.zeros(shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("args,kw,match", [
+    ((_t(2, 3, 8), _t(4, 8)), dict(activation="tanh"), "activation"),
+    ((_t(2, 3, 8, dtype=torch.float32), _t(4, 8, dtype=torch.float32)), {}, "FP16 or BF16"),
+    ((_t(2, 3, 8), _t(4, 8, dtype=torch.float16)), {}, "dtype"),
+    ((_t(8), _t(4, 8)), {}, r"\[S, K\]"),
+    ((_t(2, 3, 8), _t(4, 8)), dict(heads_in=True), "heads_in"),
+    ((_t(2, 0, 8), _t(4, 8)), {}, "nonempty"),
+    ((_t(2, 3, 8), _t(0, 8)), {}, "nonempty"),
+    ((_t(2, 3, 8), _t(4, 9)), {}, "features"),
+    ((_t(2, 2, 3, 4), _t(4, 9)), dict(heads_in=True), "features"),
+    ((_t(2, 3, 8), _t(4, 8), _t(5)), {}, "bias"),
+    ((_t(2, 3, 8), _t(4, 8), _t(4, dtype=torch.float16)), {}, "bias"),
+    ((_t(2, 3, 8), _t(4, 8)), dict(heads_out=3), "heads_out"),
+    ((_t(2, 3, 8), _t(4, 8)), dict(heads_out=True), "heads_out"),
+    ((_t(3, 8), _t(4, 8)), dict(heads_out=2), "batch axis"),
+    ((_t(2, 3, 8), _t(4, 8)), dict(heads_out=2, residual=_t(2, 3, 4)), "token-major"),
+    ((_t(2, 3, 8), _t(4, 8)), dict(gate=_t(2, 4)), "gate"),
+    ((_t(2, 3, 8), _t(4, 8)), dict(gate=_t(2, 1, 1)), "gate"),
+    ((_t(2, 3, 8), _t(4, 8)), dict(residual=_t(3, 4)), "residual"),
+    ((_t(2, 3, 8), _t(4, 8)), dict(out=_t(2, 3, 5)), "out must be"),
+    ((_t(2, 3, 8), _t(4, 8)), dict(out=_t(1, 3, 4).expand(2, 3, 4)), "overlap itself"),
+    ((_t(2, 3, 8), _t(4, 8)), dict(out=_t(2, 4, 3).transpose(1, 2)), "contiguous last axis"),
+    ((_t(2, 3, 8), _t(4, 8)), dict(status=_t(1)), "status"),
+    ((_t(2, 3, 8), _t(4, 8)), {}, "no CPU fallback"),
+])
+def test_linear_refuses(args, kw, match):
+    with pytest.raises(ValueError, match=match):
+        linear(*args, **kw)
+
+
+def test_linear_refuses_an_output_over_an_input():
+    x, w = _t(2, 3, 8), _t(8, 8)
+    with pytest.raises(ValueError, match="share memory"):
+        linear(x, w, out=x)
+    res = _t(2, 4, 8)
+    with pytest.raises(ValueError, match="share memory"):
+        linear(x, w, residual=res[:, :3], out=res[:, 1:])
+    with pytest.raises(ValueError, match="no CPU fallback"):      # in place on the residual is allowed
+        linear(x, w, residual=res[:, :3], out=res[:, :3])
+
+
+Q = _t(2, 4, 6, 16)
+TAB = _t(6, 8, dtype=torch.float32)
+
+
+@pytest.mark.parametrize("args,kw,match", [
+    ((_t(4, 6, 16), Q), {}, "q must be"),
+    ((Q, _t(2, 4, 0, 16)), {}, "k must be"),
+    ((Q, _t(2, 4, 5, 16)), {}, "match"),
+    ((Q, _t(2, 4, 6, 16, dtype=torch.float16)), {}, "dtype"),
+    ((_t(1, 1, 2, 130), _t(1, 1, 2, 130)), {}, "<= 128"),
+    ((Q, Q), dict(eps=-1.0), "eps"),
+    ((Q, Q), dict(eps=float("nan")), "eps"),
+    ((Q, Q, _t(15)), {}, "weights"),
+    ((Q, Q, _t(16, dtype=torch.float16)), {}, "weights"),
+    ((Q, Q, _t(16), _t(16, dtype=torch.float32)), {}, "share a dtype"),
+    ((Q, Q), dict(cos=TAB), "come together"),
+    ((Q, Q, None, None, TAB, _t(6, 7, dtype=torch.float32)), {}, "one shape"),
+    ((Q, Q, None, None, TAB.double(), TAB.double()), {}, "float32"),
+    ((Q, Q, None, None, _t(7, 8, dtype=torch.float32), _t(7, 8, dtype=torch.float32)), {}, "more rows"),
+    ((Q, Q, None, None, _t(6, 9, dtype=torch.float32), _t(6, 9, dtype=torch.float32)), {}, "more channels"),
+    ((Q, Q, None, None, TAB.expand(3, 6, 8), TAB.expand(3, 6, 8)), {}, "batch"),
+    ((Q, Q), dict(out=(Q,)), "out must be"),
+    ((Q, Q), dict(out=(_t(2, 4, 6, 15), _t(2, 4, 6, 16))), "q_out"),
+    ((Q, Q), {}, "no CPU fallback"),
+])
+def test_rope_refuses(args, kw, match):
+    with pytest.raises(ValueError, match=match):
+        qk_norm_rope(*args, **kw)
+
+
+def test_rope_outputs_and_inputs_in_one_buffer():
+    qkv = _t(2, 6, 3, 4, 16)
+    q, k = (qkv[:, :, i].transpose(1, 2) for i in range(2))
+    with pytest.raises(ValueError, match="no CPU fallback"):      # the parts of a fused projection, in place
+        qk_norm_rope(q, k, out=(q, k))
+    with pytest.raises(ValueError, match="share memory"):
+        qk_norm_rope(q, k, out=(k, q))
+    with pytest.raises(ValueError, match="share memory"):
+        qk_norm_rope(q, q, out=(q, q))
+
+
+def test_shares_memory_is_exact_for_equal_strides():
+    base = torch.zeros(4, 6, 8)
+    assert not _shares_memory(base[:, :3], base[:, 3:])
+    assert _shares_memory(base[:, :3], base[:, 2:5])
+    assert not _shares_memory(base[..., :4], base[..., 4:])
+    assert _shares_memory(base[..., :4], base[..., 3:7])
+    assert not _shares_memory(base[0::2], base[1::2])
+    assert _shares_memory(base[:, :3], base.transpose(0, 1)[:4, :3])      # unequal strides: by address range
+    assert _overlaps_itself(base[:1].expand(2, 6, 8)) and not _overlaps_itself(base.transpose(0, 2))
+
+
+def test_c_entries_refuse_without_a_device():
+    lib = _abi.load()
+    assert lib.vcb_linear(None, None) == _abi.VCB_ERR_INVALID_ARGUMENT
+    assert lib.vcb_linear_workspace(None) == 0
+    assert lib.vcb_qk_norm_rope(None, None) == _abi.VCB_ERR_INVALID_ARGUMENT
+    a = _abi.LinearArgs(x=16, w=16, y=16, dtype=2, batch=1, tokens=4, n=8, heads_in=1, k_head=9, x_stride_s=9,
+                        w_stride=9, n_head=8)
+    need = lib.vcb_linear_workspace(ctypes.byref(a))
+    assert need >= (4 + 8) * 16 * 2                       # both operands packed to 16 channels
+    assert lib.vcb_linear(ctypes.byref(a), None) == _abi.VCB_ERR_INVALID_ARGUMENT
+    assert "workspace" in _abi.last_error(lib)
+    a.workspace, a.workspace_bytes = 256, need - 1
+    assert lib.vcb_linear(ctypes.byref(a), None) == _abi.VCB_ERR_WORKSPACE
+    for field, value, match in [("dtype", 0, "dtype"), ("n_head", 3, "n_head"), ("activation", 9, "activation"),
+                                ("tokens", 0, "positive"), ("w_stride", 8, "overlap"), ("tokens", 1 << 31, "int32")]:
+        keep = getattr(a, field)
+        setattr(a, field, value)
+        assert lib.vcb_linear(ctypes.byref(a), None) == _abi.VCB_ERR_INVALID_ARGUMENT
+        assert match in _abi.last_error(lib)
+        setattr(a, field, keep)
+    r = _abi.QKNormRopeArgs(q=16, k=16, q_out=16, k_out=16, dtype=2, batch=1, q_heads=1, k_heads=1, tokens=4, d=8,
+                            rows=4, rotary=8, norm=1, eps=1e-6, cos=16, sin=16)
+    for field, value, match in [("d", 129, "128"), ("rotary", 7, "rotary"), ("rows", 5, "rows"), ("eps", -1.0, "eps"),
+                                ("tokens", 1 << 31, "int32"), ("sin", None, "cos")]:
+        keep = getattr(r, field)
+        setattr(r, field, value)
+        assert lib.vcb_qk_norm_rope(ctypes.byref(r), None) == _abi.VCB_ERR_INVALID_ARGUMENT
+        assert match in _abi.last_error(lib)
+        setattr(r, field, keep)

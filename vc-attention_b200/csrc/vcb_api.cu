@@ -351,6 +351,66 @@ int vcb_forward(const vcb_forward_args* a, void* stream) {
     return attn_run(&at, nullptr, st);
 }
 
+namespace {
+bool known_dtype(int t) { return t >= VCB_F32 && t <= VCB_BF16; }
+
+int check_linear(const vcb_linear_args* a) {
+    VCB_REQUIRE(a, "null argument struct");
+    VCB_REQUIRE(a->dtype == VCB_F16 || a->dtype == VCB_BF16, "dtype must be 1 (fp16) or 2 (bf16)");
+    VCB_REQUIRE(a->batch > 0 && a->tokens > 0 && a->n > 0 && a->heads_in > 0 && a->k_head > 0 && a->n_head > 0,
+                "sizes must be positive");
+    VCB_REQUIRE(a->batch < (1ll << 31) && a->tokens < (1ll << 31) && a->batch * a->tokens < (1ll << 31) - 256 &&
+                    a->n < (1ll << 31) - 256 && a->heads_in < (1ll << 24) && a->k_head < (1ll << 31) - 256 &&
+                    a->heads_in * a->k_head < (1ll << 31) - 256,
+                "sizes exceed the int32 tile counters");
+    VCB_REQUIRE(a->n % a->n_head == 0, "n_head must divide n");
+    VCB_REQUIRE(a->w_stride >= a->heads_in * a->k_head || a->n == 1, "w rows must not overlap");
+    VCB_REQUIRE(a->activation >= VCB_ACT_NONE && a->activation <= VCB_ACT_RELU, "unknown activation");
+    VCB_REQUIRE(!a->bias || known_dtype(a->bias_dtype), "unknown bias dtype");
+    VCB_REQUIRE(!a->gate || known_dtype(a->gate_dtype), "unknown gate dtype");
+    return VCB_OK;
+}
+}  // namespace
+
+size_t vcb_linear_workspace(const vcb_linear_args* a) {
+    return check_linear(a) == VCB_OK ? linear_workspace_bytes(a) : 0;
+}
+
+int vcb_linear(const vcb_linear_args* a, void* stream) {
+    int rc = check_linear(a);
+    if (rc) return rc;
+    VCB_REQUIRE(a->x && a->w && a->y, "x, w and y must be non-null");
+    const size_t need = linear_workspace_bytes(a);
+    if (need) {
+        VCB_REQUIRE(a->workspace, "workspace must be non-null");
+        VCB_REQUIRE(aligned16(a->workspace), "workspace must be 16-byte aligned");
+        if (a->workspace_bytes < need)
+            return fail(VCB_ERR_WORKSPACE, "workspace too small: %zu bytes, need %zu", a->workspace_bytes, need);
+    }
+    rc = require_sm100(nullptr);
+    if (rc) return rc;
+    return linear_run(a, static_cast<cudaStream_t>(stream));
+}
+
+int vcb_qk_norm_rope(const vcb_qk_norm_rope_args* a, void* stream) {
+    VCB_REQUIRE(a, "null argument struct");
+    VCB_REQUIRE(a->q && a->k && a->q_out && a->k_out, "q, k and their outputs must be non-null");
+    VCB_REQUIRE(known_dtype(a->dtype), "unknown dtype");
+    VCB_REQUIRE(a->batch > 0 && a->q_heads > 0 && a->k_heads > 0 && a->tokens > 0, "sizes must be positive");
+    VCB_REQUIRE(a->batch < 65536 && a->q_heads < 65536 && a->k_heads < 65536 && a->tokens < (1ll << 31) &&
+                    (a->tokens + 7) / 8 * (a->q_heads + a->k_heads) < (1ll << 31),
+                "sizes exceed the int32 grid");
+    VCB_REQUIRE(a->d >= 1 && a->d <= 128, "head dimension must be in [1, 128]");
+    VCB_REQUIRE(a->rotary >= 0 && a->rotary <= a->d && a->rotary % 2 == 0, "rotary must be even, at most d");
+    VCB_REQUIRE(a->rows >= 0 && a->rows <= a->tokens, "rows must be in [0, tokens]");
+    VCB_REQUIRE(a->rotary == 0 || a->rows == 0 || (a->cos && a->sin), "cos and sin must be non-null");
+    VCB_REQUIRE(!(a->q_weight || a->k_weight) || known_dtype(a->weight_dtype), "unknown weight dtype");
+    VCB_REQUIRE(!a->norm || (a->eps >= 0.0f && a->eps <= 3.4e38f), "eps must be finite and not negative");
+    int rc = require_sm100(nullptr);
+    if (rc) return rc;
+    return rope_run(a, static_cast<cudaStream_t>(stream));
+}
+
 int vcb_wait_selftest(int complete, const void* src, int32_t* status, int32_t* report, void* stream) {
     VCB_REQUIRE(src && report, "src and report must be non-null");
     VCB_REQUIRE(aligned16(src), "src must be 16-byte aligned");

@@ -25,6 +25,13 @@ int attn_run(const vcb_attn_args* p, const vcb_attn_probe* probe, cudaStream_t s
 int attn_exp_run(const vcb_attn_args* p, const vcb_attn_probe* probe, cudaStream_t st);
 int wait_selftest_run(int complete, const void* src, int32_t* status, int32_t* report, cudaStream_t st);
 
+// vcb_linear.cu
+size_t linear_workspace_bytes(const vcb_linear_args* a);
+int linear_run(const vcb_linear_args* a, cudaStream_t st);
+
+// vcb_rope.cu
+int rope_run(const vcb_qk_norm_rope_args* a, cudaStream_t st);
+
 // vcb_expcast.cu
 int expcast_run(const float* x, uint8_t* codes, int64_t n, cudaStream_t st);
 

@@ -4,6 +4,8 @@ Same public surface as czfsdg/vc-attention's ``vc_attention`` package
 (``Config``, ``LayoutCache``, ``attention``; src/vc_attention/__init__.py:3-5).
 """
 from .core import Config, LayoutCache, attention, to_layout_order
+from .layer import linear, qk_norm_rope
 from .streamed import attention_streamed, check_streamed
 
-__all__ = ["Config", "LayoutCache", "attention", "attention_streamed", "check_streamed", "to_layout_order"]
+__all__ = ["Config", "LayoutCache", "attention", "attention_streamed", "check_streamed", "linear", "qk_norm_rope",
+           "to_layout_order"]

@@ -71,6 +71,27 @@ class ForwardArgs(ctypes.Structure):
                 ("status", c_void_p)]
 
 
+class LinearArgs(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("w", c_void_p), ("dtype", c_int), ("batch", c_int64), ("tokens", c_int64),
+                ("n", c_int64), ("heads_in", c_int64), ("k_head", c_int64), ("x_stride_b", c_int64),
+                ("x_stride_h", c_int64), ("x_stride_s", c_int64), ("w_stride", c_int64), ("bias", c_void_p),
+                ("bias_dtype", c_int), ("activation", c_int), ("gate", c_void_p), ("gate_dtype", c_int),
+                ("gate_stride_b", c_int64), ("gate_stride_s", c_int64), ("residual", c_void_p),
+                ("residual_stride_b", c_int64), ("residual_stride_s", c_int64), ("y", c_void_p), ("n_head", c_int64),
+                ("y_stride_b", c_int64), ("y_stride_h", c_int64), ("y_stride_s", c_int64), ("status", c_void_p),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
+class QKNormRopeArgs(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p), ("dtype", c_int),
+                ("batch", c_int64), ("q_heads", c_int64), ("k_heads", c_int64), ("tokens", c_int64), ("d", c_int),
+                ("q_stride", c_int64 * 3), ("k_stride", c_int64 * 3), ("q_out_stride", c_int64 * 3),
+                ("k_out_stride", c_int64 * 3), ("q_weight", c_void_p), ("k_weight", c_void_p),
+                ("weight_dtype", c_int), ("cos", c_void_p), ("sin", c_void_p), ("rows", c_int64), ("rotary", c_int),
+                ("table_stride_b", c_int64), ("table_stride_s", c_int64), ("interleaved", c_int), ("norm", c_int),
+                ("eps", c_float)]
+
+
 # name -> (restype, argtypes); every symbol include/vcb.h declares.
 SIGNATURES = {
     "vcb_abi_version": (c_int, []),
@@ -91,6 +112,9 @@ SIGNATURES = {
     "vcb_attention_fp8_probe": (c_int, [ctypes.POINTER(AttnArgs), ctypes.POINTER(AttnProbe), c_void_p]),
     "vcb_forward_workspace": (c_size_t, [ctypes.POINTER(ForwardArgs)]),
     "vcb_forward": (c_int, [ctypes.POINTER(ForwardArgs), c_void_p]),
+    "vcb_linear_workspace": (c_size_t, [ctypes.POINTER(LinearArgs)]),
+    "vcb_linear": (c_int, [ctypes.POINTER(LinearArgs), c_void_p]),
+    "vcb_qk_norm_rope": (c_int, [ctypes.POINTER(QKNormRopeArgs), c_void_p]),
     "vcb_read_status": (c_int, [c_void_p, c_void_p, ctypes.POINTER(ctypes.c_int32)]),
     "vcb_wait_selftest": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
 }
