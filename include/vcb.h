@@ -230,7 +230,7 @@ VCB_API size_t vcb_forward_workspace(const vcb_forward_args* args);
  * scale, k_smooth, hadamard) (bindings.cpp:100-178) */
 VCB_API int vcb_forward(const vcb_forward_args* args, void* stream);
 
-/* ---- around the attention: projections, Q/K norm and rotation ------------------
+/* ---- around the attention: projections, Q/K norm and rotation, window ----------
  * These entry points have no reference counterpart: the reference receives
  * post-RoPE Q/K/V from the model (core.py:243-262).  Tensors are addressed by
  * strides in elements; the last axis is contiguous.  Non-finite values pass
@@ -301,6 +301,34 @@ typedef struct {
 } vcb_qk_norm_rope_args;
 
 VCB_API int vcb_qk_norm_rope(const vcb_qk_norm_rope_args* args, void* stream);
+
+/* 16-bit attention over a sliding window.  Query i stands at position
+ * p = i + offset (q_offset, or without has_offset the entry's keys - sq, which
+ * puts the last query on the last key) and sees key j < keys of its batch entry
+ * when (j < sinks or p - left <= j <= p + right) and (not causal or j <= p).
+ * out = softmax(scale q . k) v over the seen keys; a row that sees none is 0.
+ * Keys that no row sees do not reach the output, whatever they hold. */
+typedef struct {
+    const void* q; const void* k; const void* v;
+    void* out;
+    int dtype;                      /* VCB_F16 or VCB_BF16 */
+    int64_t batch, heads, sq, sk;
+    int d;                          /* 1..128 */
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];   /* batch, head, token */
+    const int32_t* kv_lens;         /* [batch] keys of each entry, clamped to 0..sk on the device, or NULL: sk */
+    int64_t left, right;            /* -1: no bound */
+    int64_t sinks;
+    int causal;
+    int has_offset;
+    int64_t q_offset;
+    float scale;                    /* positive, finite */
+    int32_t* status;                /* device status word (nullable); flags are ORed in */
+    void* workspace;
+    size_t workspace_bytes;
+} vcb_window_args;
+
+VCB_API size_t vcb_window_workspace(const vcb_window_args* args);
+VCB_API int vcb_window_attention(const vcb_window_args* args, void* stream);
 
 /* Reads the device status word into *flags: one device-to-host copy ordered
  * on `stream` (not on the legacy default stream), then a wait for `stream`

@@ -4,7 +4,7 @@ import ctypes
 import pytest
 import torch
 
-from vc_attention_b200 import _abi, linear, qk_norm_rope
+from vc_attention_b200 import _abi, linear, qk_norm_rope, window_attention
 from vc_attention_b200.layer import _overlaps_itself, _shares_memory
 
 BF16 = torch.bfloat16
@@ -136,3 +136,49 @@ def test_c_entries_refuse_without_a_device():
         assert lib.vcb_qk_norm_rope(ctypes.byref(r), None) == _abi.VCB_ERR_INVALID_ARGUMENT
         assert match in _abi.last_error(lib)
         setattr(r, field, keep)
+
+
+W = _t(2, 3, 5, 16)
+
+
+@pytest.mark.parametrize("args,kw,match", [
+    ((_t(3, 5, 16), W, W), {}, "BNSD"),
+    ((W, _t(2, 4, 5, 16), _t(2, 4, 5, 16)), {}, "Incompatible"),
+    ((W, W, _t(2, 3, 6, 16)), {}, "Incompatible"),
+    ((W, _t(2, 3, 5, 8), _t(2, 3, 5, 8)), {}, "Incompatible"),
+    ((_t(2, 3, 0, 16), W, W), {}, "Empty"),
+    ((W, W, W.half()), {}, "dtype"),
+    ((W.float(), W.float(), W.float()), {}, "FP16 or BF16"),
+    ((_t(1, 1, 2, 129), _t(1, 1, 2, 129), _t(1, 1, 2, 129)), {}, "<= 128"),
+    ((W, W, W), dict(window=(1, 2, 3)), "window"),
+    ((W, W, W), dict(window=(-1, 0)), "left"),
+    ((W, W, W), dict(window=(1, 1.5)), "right"),
+    ((W, W, W), dict(sinks=-1), "sinks"),
+    ((W, W, W), dict(sinks=None), "sinks"),
+    ((W, W, W), dict(q_offset=1.0), "q_offset"),
+    ((W, W, W), dict(kv_lens=torch.zeros(2, dtype=torch.int64)), "kv_lens"),
+    ((W, W, W), dict(kv_lens=torch.zeros(3, dtype=torch.int32)), "kv_lens"),
+    ((W, W, W), dict(scale=0.0), "scale"),
+    ((W, W, W), dict(scale=float("inf")), "scale"),
+    ((W, W, W), dict(out=W), "share memory"),
+    ((W, W, W), dict(status=_t(2, dtype=torch.int32)), "status"),
+    ((W, W, W), {}, "no CPU fallback"),
+])
+def test_window_refuses(args, kw, match):
+    with pytest.raises(ValueError, match=match):
+        window_attention(*args, **kw)
+
+
+def test_window_c_entry_refuses_without_a_device():
+    lib = _abi.load()
+    assert lib.vcb_window_attention(None, None) == _abi.VCB_ERR_INVALID_ARGUMENT
+    a = _abi.WindowArgs(q=16, k=16, v=16, out=16, dtype=2, batch=1, heads=1, sq=4, sk=4, d=16, left=-1, right=-1,
+                        scale=1.0)
+    for field, value, match in [("dtype", 0, "dtype"), ("d", 200, "128"), ("left", -2, "window"), ("sinks", -1, "sinks"),
+                                ("scale", -1.0, "scale"), ("sk", 1 << 31, "int32"), ("heads", 70000, "int32"),
+                                ("out", None, "non-null")]:
+        keep = getattr(a, field)
+        setattr(a, field, value)
+        assert lib.vcb_window_attention(ctypes.byref(a), None) == _abi.VCB_ERR_INVALID_ARGUMENT
+        assert match in _abi.last_error(lib)
+        setattr(a, field, keep)

@@ -411,6 +411,45 @@ int vcb_qk_norm_rope(const vcb_qk_norm_rope_args* a, void* stream) {
     return rope_run(a, static_cast<cudaStream_t>(stream));
 }
 
+namespace {
+int check_window(const vcb_window_args* a) {
+    VCB_REQUIRE(a, "null argument struct");
+    VCB_REQUIRE(a->dtype == VCB_F16 || a->dtype == VCB_BF16, "dtype must be 1 (fp16) or 2 (bf16)");
+    VCB_REQUIRE(a->batch > 0 && a->heads > 0 && a->sq > 0 && a->sk > 0, "sizes must be positive");
+    VCB_REQUIRE(a->batch < 65536 && a->heads < 65536 && a->batch * a->heads < 65536 && a->sq < (1ll << 31) - 256 &&
+                    a->sk < (1ll << 31) - 256,
+                "sizes exceed the int32 grid");
+    VCB_REQUIRE(a->d >= 1 && a->d <= 128, "head dimension must be in [1, 128]");
+    const int64_t far = 1ll << 40;
+    VCB_REQUIRE(a->left >= -1 && a->left < far && a->right >= -1 && a->right < far,
+                "window bounds must be non-negative, or -1 for none");
+    VCB_REQUIRE(a->sinks >= 0 && a->sinks < far, "sinks must be non-negative");
+    VCB_REQUIRE(!a->has_offset || (a->q_offset > -far && a->q_offset < far), "q_offset is out of range");
+    VCB_REQUIRE(a->scale > 0.0f && a->scale <= 3.4e38f, "scale must be positive and finite");
+    return VCB_OK;
+}
+}  // namespace
+
+size_t vcb_window_workspace(const vcb_window_args* a) {
+    return check_window(a) == VCB_OK ? window_workspace_bytes(a) : 0;
+}
+
+int vcb_window_attention(const vcb_window_args* a, void* stream) {
+    int rc = check_window(a);
+    if (rc) return rc;
+    VCB_REQUIRE(a->q && a->k && a->v && a->out, "q, k, v and out must be non-null");
+    const size_t need = window_workspace_bytes(a);
+    if (need) {
+        VCB_REQUIRE(a->workspace, "workspace must be non-null");
+        VCB_REQUIRE(aligned16(a->workspace), "workspace must be 16-byte aligned");
+        if (a->workspace_bytes < need)
+            return fail(VCB_ERR_WORKSPACE, "workspace too small: %zu bytes, need %zu", a->workspace_bytes, need);
+    }
+    rc = require_sm100(nullptr);
+    if (rc) return rc;
+    return window_run(a, static_cast<cudaStream_t>(stream));
+}
+
 int vcb_wait_selftest(int complete, const void* src, int32_t* status, int32_t* report, void* stream) {
     VCB_REQUIRE(src && report, "src and report must be non-null");
     VCB_REQUIRE(aligned16(src), "src must be 16-byte aligned");

@@ -32,6 +32,10 @@ int linear_run(const vcb_linear_args* a, cudaStream_t st);
 // vcb_rope.cu
 int rope_run(const vcb_qk_norm_rope_args* a, cudaStream_t st);
 
+// vcb_window.cu
+size_t window_workspace_bytes(const vcb_window_args* a);
+int window_run(const vcb_window_args* a, cudaStream_t st);
+
 // vcb_expcast.cu
 int expcast_run(const float* x, uint8_t* codes, int64_t n, cudaStream_t st);
 

@@ -6,6 +6,7 @@ Same public surface as czfsdg/vc-attention's ``vc_attention`` package
 from .core import Config, LayoutCache, attention, to_layout_order
 from .layer import linear, qk_norm_rope
 from .streamed import attention_streamed, check_streamed
+from .window import window_attention
 
 __all__ = ["Config", "LayoutCache", "attention", "attention_streamed", "check_streamed", "linear", "qk_norm_rope",
-           "to_layout_order"]
+           "to_layout_order", "window_attention"]

@@ -92,6 +92,15 @@ class QKNormRopeArgs(ctypes.Structure):
                 ("eps", c_float)]
 
 
+class WindowArgs(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("dtype", c_int),
+                ("batch", c_int64), ("heads", c_int64), ("sq", c_int64), ("sk", c_int64), ("d", c_int),
+                ("q_stride", c_int64 * 3), ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3),
+                ("out_stride", c_int64 * 3), ("kv_lens", c_void_p), ("left", c_int64), ("right", c_int64),
+                ("sinks", c_int64), ("causal", c_int), ("has_offset", c_int), ("q_offset", c_int64),
+                ("scale", c_float), ("status", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
 # name -> (restype, argtypes); every symbol include/vcb.h declares.
 SIGNATURES = {
     "vcb_abi_version": (c_int, []),
@@ -115,6 +124,8 @@ SIGNATURES = {
     "vcb_linear_workspace": (c_size_t, [ctypes.POINTER(LinearArgs)]),
     "vcb_linear": (c_int, [ctypes.POINTER(LinearArgs), c_void_p]),
     "vcb_qk_norm_rope": (c_int, [ctypes.POINTER(QKNormRopeArgs), c_void_p]),
+    "vcb_window_workspace": (c_size_t, [ctypes.POINTER(WindowArgs)]),
+    "vcb_window_attention": (c_int, [ctypes.POINTER(WindowArgs), c_void_p]),
     "vcb_read_status": (c_int, [c_void_p, c_void_p, ctypes.POINTER(ctypes.c_int32)]),
     "vcb_wait_selftest": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
 }

@@ -1,0 +1,95 @@
+"""Attention over a sliding window with first tokens that stay visible.
+
+The companion of ``attention`` for layers that look at a part of the sequence:
+the neighbourhood of each token, and optionally the first tokens (for a
+streamed video, the first frame).  It computes in 16-bit operands with FP32
+accumulation, with no quantisation, clustering or schedule."""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _abi
+from .b200_backend import _DTYPES, _extension, _require_b200, _stream
+from .layer import _check_out, _check_status, _ptr, _rows
+
+
+def _bound(value, name):
+    if value is None:
+        return -1
+    if isinstance(value, bool) or not isinstance(value, int) or value < 0:
+        raise ValueError(f"{name} must be a non-negative integer or None")
+    return min(value, 1 << 39)
+
+
+@torch.no_grad()
+def window_attention(q, k, v, *, window=(None, None), sinks=0, causal=False, q_offset=None, kv_lens=None, scale=None,
+                     out=None, status=None):
+    """softmax(scale * q @ k.T) @ v over the keys that each query sees.
+
+    ``q`` is [B, H, Sq, D], ``k`` and ``v`` are [B, H, Sk, D]: FP16 or BF16,
+    D <= 128, any strides (for example rows of a longer cache).  Query i stands
+    at position p = i + ``q_offset``; by default the last query stands on the
+    last key.  It sees key j when ``(j < sinks or p - left <= j <= p + right)
+    and (not causal or j <= p)``, with ``window=(left, right)`` and None for no
+    bound.  ``kv_lens``: an int32 CUDA tensor [B] with each batch entry's number
+    of keys (values are clamped to 0..Sk; whatever the padding behind it holds,
+    it does not reach the output).  A query that sees no key gives zeros.
+    ``scale`` defaults to D ** -0.5.
+
+    Returns [B, H, Sq, D], or writes ``out``, which shares no memory with an
+    input.  The call only queues work; ``status`` is as for ``linear``."""
+    if any(t.ndim != 4 for t in (q, k, v)):
+        raise ValueError("Expected BNSD tensors")
+    if q.shape[:2] != k.shape[:2] or k.shape != v.shape or q.shape[3] != k.shape[3]:
+        raise ValueError("Incompatible Q/K/V shape; batch, heads and head dimension must match")
+    if any(0 in t.shape for t in (q, k, v)):
+        raise ValueError("Empty Q/K/V are not supported")
+    if any(t.device != q.device or t.dtype != q.dtype for t in (k, v)):
+        raise ValueError("Q/K/V must have the same device and dtype")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("window_attention takes FP16 or BF16 inputs")
+    b, h, sq, d = q.shape
+    if d > 128:
+        raise ValueError("window_attention supports head dimensions <= 128")
+    if len(window) != 2:
+        raise ValueError("window must be (left, right)")
+    left, right = _bound(window[0], "left"), _bound(window[1], "right")
+    if sinks is None:
+        raise ValueError("sinks must be a non-negative integer")
+    first = _bound(sinks, "sinks")
+    if q_offset is not None and (isinstance(q_offset, bool) or not isinstance(q_offset, int) or
+                                 abs(q_offset) >= 1 << 39):
+        raise ValueError("q_offset must be an integer position")
+    if kv_lens is not None and (kv_lens.dtype != torch.int32 or tuple(kv_lens.shape) != (b,) or
+                                kv_lens.device != q.device):
+        raise ValueError("kv_lens must be an int32 tensor [B] on the inputs' device")
+    scale = d ** -0.5 if scale is None else scale
+    if not math.isfinite(scale) or scale <= 0:
+        raise ValueError("scale must be positive and finite")
+    _check_status(status, q.device)
+    if out is not None:
+        _check_out(out, q.shape, q, "out", (q, k, v, kv_lens))
+    _require_b200(q, "window_attention")
+    lib = _extension()
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if kv_lens is not None:
+        kv_lens = kv_lens.contiguous()
+    triple = ctypes.c_int64 * 3
+    a = _abi.WindowArgs(
+        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), dtype=_DTYPES[q.dtype], batch=b, heads=h,
+        sq=sq, sk=k.shape[2], d=d, q_stride=triple(*q.stride()[:3]), k_stride=triple(*k.stride()[:3]),
+        v_stride=triple(*v.stride()[:3]), out_stride=triple(*out.stride()[:3]), kv_lens=_ptr(kv_lens), left=left,
+        right=right, sinks=first, causal=int(bool(causal)), has_offset=int(q_offset is not None),
+        q_offset=q_offset or 0, scale=float(scale), status=_ptr(status))
+    need = lib.vcb_window_workspace(ctypes.byref(a))
+    if need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), need
+    with torch.cuda.device(q.device):
+        _abi.check(lib, lib.vcb_window_attention(ctypes.byref(a), _stream(q.device)))
+    return out
