@@ -425,7 +425,7 @@ int check_window(const vcb_window_args* a) {
                 "window bounds must be non-negative, or -1 for none");
     VCB_REQUIRE(a->sinks >= 0 && a->sinks < far, "sinks must be non-negative");
     VCB_REQUIRE(!a->has_offset || (a->q_offset > -far && a->q_offset < far), "q_offset is out of range");
-    VCB_REQUIRE(a->scale > 0.0f && a->scale <= 3.4e38f, "scale must be positive and finite");
+    VCB_REQUIRE(a->scale >= 1e-30f && a->scale <= 1e30f, "scale must be in [1e-30, 1e30]");
     return VCB_OK;
 }
 }  // namespace

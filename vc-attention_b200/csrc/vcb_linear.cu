@@ -31,9 +31,7 @@
 //
 // Every mbarrier wait is bounded (vcb_attn_pair.cuh); a CTA that gives up
 // tells its peer, and the pair drains and frees its tensor memory together.
-#include <cstring>
-
-#include "vcb_attn_pair.cuh"
+#include "vcb_f16.cuh"
 
 namespace vcb {
 namespace {
@@ -98,16 +96,6 @@ __device__ __forceinline__ void mma2_f16(uint32_t d_tmem, uint32_t a_lo, uint32_
         "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %4, p;\n\t}"
         ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
         : "memory");
-}
-
-// Instruction descriptor, kind::f16: F32 D (c_format [4,6) = 1), A and B both
-// FP16 (0) or both BF16 (1) at [7,10) and [10,13), both K-major.
-template <typename T> __host__ __device__ constexpr uint32_t idesc_f16(int m, int n);
-template <> __host__ __device__ constexpr uint32_t idesc_f16<__half>(int m, int n) {
-    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-template <> __host__ __device__ constexpr uint32_t idesc_f16<__nv_bfloat16>(int m, int n) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 struct LinBars {
@@ -254,24 +242,6 @@ __device__ __forceinline__ void load8_any(const void* p, int64_t i, int dtype, i
     }
 }
 
-template <typename T> struct Pack8;
-template <> struct Pack8<__half> {
-    static constexpr int kDtype = VCB_F16;
-    static __device__ __forceinline__ __half one(float f) { return __float2half_rn(f); }
-    static __device__ __forceinline__ uint32_t two(float a, float b) {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-};
-template <> struct Pack8<__nv_bfloat16> {
-    static constexpr int kDtype = VCB_BF16;
-    static __device__ __forceinline__ __nv_bfloat16 one(float f) { return __float2bfloat16_rn(f); }
-    static __device__ __forceinline__ uint32_t two(float a, float b) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-};
-
 // Eight accumulated columns n .. n + 7 of one row: act, gate, residual, store.
 // f holds the sums with the bias added.
 template <typename T>
@@ -290,7 +260,7 @@ __device__ __forceinline__ void finish8(const LinParams& p, float* f, int n, int
     }
     if (p.residual) {
         float q[8];
-        load8_any(p.residual, r_off + n, Pack8<T>::kDtype, valid, p.vec_r, q);
+        load8_any(p.residual, r_off + n, F16<T>::kDtype, valid, p.vec_r, q);
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = __fadd_rn(f[e], q[e]);
     }
@@ -298,14 +268,14 @@ __device__ __forceinline__ void finish8(const LinParams& p, float* f, int n, int
     if (p.vec_y && valid >= 8) {
         const int h = n / p.n_head;
         *reinterpret_cast<uint4*>(y + h * p.ys_h + (n - h * p.n_head)) =
-            make_uint4(Pack8<T>::two(f[0], f[1]), Pack8<T>::two(f[2], f[3]), Pack8<T>::two(f[4], f[5]),
-                       Pack8<T>::two(f[6], f[7]));
+            make_uint4(F16<T>::two(f[0], f[1]), F16<T>::two(f[2], f[3]), F16<T>::two(f[4], f[5]),
+                       F16<T>::two(f[6], f[7]));
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             if (e < valid) {
                 const int h = (n + e) / p.n_head;
-                y[h * p.ys_h + (n + e - h * p.n_head)] = Pack8<T>::one(f[e]);
+                y[h * p.ys_h + (n + e - h * p.n_head)] = F16<T>::one(f[e]);
             }
     }
 }
@@ -439,52 +409,6 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_kernel(const __grid_con
     if (threadIdx.x == 0 && *abort) flag_status(p.status, VCB_FLAG_TIMEOUT);
 }
 
-// Rows of `channels` elements (heads x channels per row, strides in elements)
-// into rows of `pitch` elements, zero behind the last channel.
-struct PackSide {
-    const uint16_t* src;
-    uint16_t* dst;
-    int64_t rows, tokens;                 // row r is (r / tokens, r % tokens)
-    int64_t s_b, s_h, s_s;
-    int head_dim;
-};
-struct PackParams {
-    PackSide side[2];
-    int64_t blocks0;                      // blocks of side 0
-    int channels, pitch;
-};
-__global__ void __launch_bounds__(256) linear_pack_kernel(const __grid_constant__ PackParams p) {
-    pdl_wait();
-    pdl_open();
-    const int which = blockIdx.x >= p.blocks0;
-    const PackSide& s = p.side[which];
-    const int64_t row = ((int64_t)blockIdx.x - (which ? p.blocks0 : 0)) * 8 + (threadIdx.x >> 5);
-    if (row >= s.rows) return;
-    const int64_t b = row / s.tokens, t = row - b * s.tokens;
-    const uint16_t* src = s.src + b * s.s_b + t * s.s_s;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(s.dst + row * p.pitch);
-    auto get = [&](int c) -> uint32_t {
-        if (c >= p.channels) return 0u;
-        const int h = c / s.head_dim;
-        return src[h * s.s_h + (c - h * s.head_dim)];
-    };
-    for (int c = 2 * (threadIdx.x & 31); c < p.pitch; c += 64) dst[c / 2] = get(c) | (get(c + 1) << 16);
-}
-
-int make_map16(CUtensorMap* map, const void* base, bool bf16, int rank, const cuuint64_t* dims,
-               const cuuint64_t* strides, const cuuint32_t* box) {
-    EncodeTiledFn enc;
-    int rc = get_encoder(&enc);
-    if (rc) return rc;
-    const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-    CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
-                     const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(VCB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-    return VCB_OK;
-}
-
 template <typename T, int BN>
 int launch_tiles(LinParams& p, cudaStream_t st) {
     static int max_pairs[64] = {};
@@ -522,9 +446,6 @@ int launch_tiles(LinParams& p, cudaStream_t st) {
     return VCB_OK;
 }
 
-bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-bool by8(int64_t v) { return v % 8 == 0; }
-
 struct LinPlan {
     bool pack_x, pack_w;
     int64_t pitch;               // elements of a packed row
@@ -535,11 +456,9 @@ LinPlan plan(const vcb_linear_args* a) {
     LinPlan q{};
     const int64_t k = a->heads_in * a->k_head;
     q.pitch = (k + 7) / 8 * 8;
-    // TMA: 16-byte bases and strides; a stride of zero or below is not addressed
-    auto stride_ok = [](int64_t s, int64_t n) { return n == 1 || (by8(s) && s > 0); };
-    q.pack_w = !on16(a->w) || !stride_ok(a->w_stride, a->n);
-    q.pack_x = !on16(a->x) || (a->heads_in > 1 && !by8(a->k_head)) || !stride_ok(a->x_stride_s, a->tokens) ||
-               !stride_ok(a->x_stride_h, a->heads_in) || !stride_ok(a->x_stride_b, a->batch);
+    q.pack_w = !on16(a->w) || !tma_stride(a->w_stride, a->n);
+    q.pack_x = !on16(a->x) || (a->heads_in > 1 && !by8(a->k_head)) || !tma_stride(a->x_stride_s, a->tokens) ||
+               !tma_stride(a->x_stride_h, a->heads_in) || !tma_stride(a->x_stride_b, a->batch);
     auto r = [](size_t v) { return (v + 255) & ~size_t(255); };
     q.off_w = q.pack_x ? r((size_t)(a->batch * a->tokens * q.pitch) * 2) : 0;
     q.total = q.off_w + (q.pack_w ? r((size_t)(a->n * q.pitch) * 2) : 0);
@@ -562,24 +481,26 @@ int linear_run(const vcb_linear_args* a, cudaStream_t st) {
         pk.channels = (int)k;
         pk.pitch = (int)q.pitch;
         char* ws = static_cast<char*>(a->workspace);
+        int64_t blocks = 0;
         if (q.pack_x) {
             const int64_t rows = a->batch * a->tokens;
-            pk.side[0] = {static_cast<const uint16_t*>(x), reinterpret_cast<uint16_t*>(ws), rows, a->tokens, xb, xh, xs,
-                          (int)a->k_head};
-            pk.blocks0 = (rows + 7) / 8;
+            pk.side[0] = {static_cast<const uint16_t*>(x), reinterpret_cast<uint16_t*>(ws), rows, a->tokens, xb, xs, 1,
+                          0, xh, (int)a->k_head};
+            blocks += (rows + 7) / 8;
             x = ws;
             xs = q.pitch; xh = k; xb = a->tokens * q.pitch;
         }
-        int64_t blocks = pk.blocks0;
+        pk.end[0] = blocks;
         if (q.pack_w) {
-            pk.side[1] = {static_cast<const uint16_t*>(w), reinterpret_cast<uint16_t*>(ws + q.off_w), a->n, a->n, 0, k,
-                          a->w_stride, (int)k};
+            pk.side[1] = {static_cast<const uint16_t*>(w), reinterpret_cast<uint16_t*>(ws + q.off_w), a->n, a->n, 0,
+                          a->w_stride, 1, 0, k, (int)k};
             blocks += (a->n + 7) / 8;
             w = ws + q.off_w;
             w_stride = q.pitch;
         }
+        pk.end[1] = pk.end[2] = blocks;
         if (q.pack_x) { heads = 1; k_head = k; }      // a packed row has its heads joined
-        VCB_CUDA(launch_pdl(linear_pack_kernel, dim3((unsigned)blocks), dim3(256), 0, st, pk));
+        VCB_CUDA(launch_pack(pk, st));
     }
     LinParams p;
     memset(&p, 0, sizeof(p));

@@ -3,13 +3,46 @@
 // keys when
 //   (j < sinks or p - left <= j <= p + right) and (not causal or j <= p);
 // out = softmax over the seen keys of (scale q . k), times v; 0 for a row that
-// sees none.  The seen keys are two runs, [0, sink) and [lo, hi).
-#include "vcb_internal.h"
+// sees none.  The seen keys are two runs, [0, sink) and [lo, hi), so a CTA
+// walks the 128-key tiles of two runs and skips all others.
+//
+// Bound: the tensor cores (4 D operations a pair) and the exponentials (16 a
+// clock and SM: as long as the two products of a 128-wide head), for few
+// queries the bytes of K and V.
+//
+// Work decomposition.  A CTA owns NQ (1 or 2) tiles of 128 queries of one
+// head, and with few queries one of `splits` parts of their key tiles; parts
+// are joined by window_join_kernel in a fixed order.  Per key tile and query
+// tile: S = Q K^T into tensor memory (tcgen05, 128 x 128), the softmax
+// warpgroup of the query tile (one thread per row) turns S into P = 2^(s - m)
+// in 16 bits over S's own columns, and O += P V adds onto the row's sums in
+// tensor memory.  V stays [key][channel] as it comes: it is the N-major B
+// operand.  With two query tiles one tile's products run under the other's
+// softmax; the issue order PV_0(j), QK_0(j+1), PV_1(j), QK_1(j+1) makes S_w(j+1)
+// follow P_w(j) in the same columns without a further wait.
+//
+// The running maximum moves only when a row's maximum passes it by 2^8: until
+// then P just grows, exactly representable in FP32 sums and both 16-bit types,
+// and O is not rescaled.  A softmax warp rescales O itself, between the commit
+// that follows PV_w(j-1) and its own arrival for PV_w(j).  The row sum adds the
+// rounded P, so the weights are normalised as they are used.
+//
+// A masked key has P = 0, but 0 times a NaN or infinity in its V row would
+// still reach O.  Rows behind a batch entry's last key are therefore cleared in
+// shared memory, and a row whose sums are not finite is computed again by
+// window_row, which reads only the keys that the row sees.
+//
+// Roles (128 + 128 NQ threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2
+// clears V rows behind the last key, warp 3 tensor memory; then one softmax
+// warpgroup per query tile, which also writes the output.  Every mbarrier wait
+// is bounded; a CTA that gives up drains and frees its tensor memory.
+#include "vcb_f16.cuh"
 
 namespace vcb {
 namespace {
 
 struct WinParams {
+    CUtensorMap tm_q, tm_k, tm_v;            // [batch][head][token][channel]
     const void* q;
     const void* k;
     const void* v;
@@ -20,6 +53,11 @@ struct WinParams {
     int64_t left, right, sinks, q_offset;
     int causal, has_offset, d;
     float scale;
+    float c;                                 // scale log2(e)
+    int q_tiles, splits, vec_out;
+    float* part;                             // [splits][batch heads][sq][HD] sums, splits > 1
+    float2* part_ml;                         // [splits][batch heads][sq] maximum (log2) and row sum
+    int32_t* status;
 };
 
 // The keys that the query at position p sees: [0, sink) and [lo, hi), lo >= sink.
@@ -46,12 +84,6 @@ __device__ __forceinline__ int64_t keys_of(const WinParams& p, int64_t b) {
     return n < 0 ? 0 : n > p.sk ? p.sk : n;
 }
 
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_f(float f);
-template <> __device__ __forceinline__ __half from_f<__half>(float f) { return __float2half_rn(f); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float f) { return __float2bfloat16_rn(f); }
-
 // One output row by one warp, reading only the keys that the row sees: lane l
 // takes every 32nd key's logit, then channels l, l + 32, ... of the sum.
 // `qrow` is 128 floats of shared memory of this warp.
@@ -63,7 +95,7 @@ __device__ void window_row(const WinParams& p, int64_t b, int64_t h, int64_t i, 
     const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + h * p.ks[1];
     const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + h * p.vs[1];
     __syncwarp();
-    for (int c = lane; c < 128; c += 32) qrow[c] = c < p.d ? to_f(q[c]) : 0.0f;
+    for (int c = lane; c < 128; c += 32) qrow[c] = c < p.d ? F16<T>::to(q[c]) : 0.0f;
     __syncwarp();
     float m = -INFINITY, den = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int part = 0; part < 2; ++part) {
@@ -74,7 +106,7 @@ __device__ void window_row(const WinParams& p, int64_t b, int64_t h, int64_t i, 
             if (lane < n) {
                 const T* row = k + (int64_t)(base + lane) * p.ks[2];
                 float dot = 0.0f;
-                for (int c = 0; c < p.d; ++c) dot = __fmaf_rn(qrow[c], to_f(row[c]), dot);
+                for (int c = 0; c < p.d; ++c) dot = __fmaf_rn(qrow[c], F16<T>::to(row[c]), dot);
                 logit = __fmul_rn(dot, p.scale);
             }
             float top = logit;
@@ -95,7 +127,7 @@ __device__ void window_row(const WinParams& p, int64_t b, int64_t h, int64_t i, 
                 const T* row = v + (int64_t)(base + j) * p.vs[2];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (lane + 32 * e < p.d) acc[e] = __fmaf_rn(wj, to_f(row[lane + 32 * e]), acc[e]);
+                    if (lane + 32 * e < p.d) acc[e] = __fmaf_rn(wj, F16<T>::to(row[lane + 32 * e]), acc[e]);
             }
             m = m_new;
         }
@@ -103,26 +135,587 @@ __device__ void window_row(const WinParams& p, int64_t b, int64_t h, int64_t i, 
     T* out = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + i * p.os[2];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (lane + 32 * e < p.d) out[lane + 32 * e] = from_f<T>(den == 0.0f ? 0.0f : acc[e] / den);
+        if (lane + 32 * e < p.d) out[lane + 32 * e] = F16<T>::one(den == 0.0f ? 0.0f : acc[e] / den);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) window_row_kernel(const __grid_constant__ WinParams p) {
+constexpr int kKT = 128;                           // keys per tile
+
+template <int HD, int NQ> struct WinTile {
+    static constexpr int kBoxes = HD / 64;                       // 64-channel (128-byte) boxes of a row
+    static constexpr uint32_t kBox = 128 * 128;                  // 128 rows of a box
+    static constexpr uint32_t kBytes = kBoxes * kBox;            // one Q, K or V tile
+    static constexpr int kStages = NQ == 2 ? (HD == 128 ? 5 : 8) : (HD == 128 ? 2 : 5);
+    static constexpr uint32_t kOffKV = NQ * kBytes;
+    static constexpr uint32_t kOffBars = kOffKV + kStages * kBytes;
+    static constexpr int kNumBars = 1 + 2 * kStages + 3 * 2 + 1 + 1;
+    static constexpr uint32_t kOffMisc = kOffBars + kNumBars * 8;
+    static constexpr uint32_t kSmem = kOffMisc + 16;
+    static constexpr int kThreads = 128 + 128 * NQ;
+    static constexpr int kCtas = NQ == 2 ? 1 : 2;                // per SM
+    // tensor memory: S (P over it) and O of each query tile
+    static constexpr uint32_t kCols = NQ == 2 ? 512 : 256;
+    static constexpr uint32_t kColO = NQ * 128;
+    // setmaxnreg shares: control warps, softmax warps
+    static constexpr int kRegsCtl = NQ == 2 ? 80 : 64, kRegsSoft = NQ == 2 ? 208 : 192;
+    static constexpr int kRegSplit = 128 * kRegsCtl + 128 * NQ * kRegsSoft;
+    static_assert(kSmem <= 232448 / kCtas - (kCtas - 1) * 1024, "shared memory of one CTA");
+};
+
+struct WinBars {
+    uint64_t* q_full;
+    uint64_t* kv_full;    // [stages]
+    uint64_t* kv_empty;   // [stages]  the stage's products are done
+    uint64_t* s_full;     // [2]  S_w(j) is there, and PV_w(j-1) done
+    uint64_t* p_full;     // [2]  P_w(j) is there, O_w rescaled
+    uint64_t* o_full;     // [2]  the last PV_w is done
+    uint64_t* v_last;     // [1]  the V tile that holds the last key landed; warp 2 clears the rows behind it
+                          //      and arrives on that stage's kv_full itself
+    uint64_t* drain;      // [1]
+};
+template <typename L> __device__ __forceinline__ WinBars win_bars(uint8_t* smem) {
+    uint64_t* b = reinterpret_cast<uint64_t*>(smem + L::kOffBars);
+    WinBars r;
+    r.q_full = b; b += 1;
+    r.kv_full = b; b += L::kStages;
+    r.kv_empty = b; b += L::kStages;
+    r.s_full = b; b += 2;
+    r.p_full = b; b += 2;
+    r.o_full = b; b += 2;
+    r.v_last = b; b += 1;
+    r.drain = b;
+    return r;
+}
+
+// What a CTA works on: queries [row0, row0 + 128 nq) of head (b, h) and the
+// key tiles begin .. begin + count - 1 of its list, tiles 0 .. n1 - 1 and then
+// from w0 on.
+struct WinItem {
+    int64_t b, h, bh, row0, len, offset;
+    int split, nq, n1, w0, begin, count;
+    __device__ __forceinline__ int tile(int j) const {
+        const int i = begin + j;
+        return i < n1 ? i : w0 + i - n1;
+    }
+};
+template <int NQ> __device__ __forceinline__ WinItem win_item(const WinParams& p) {
+    WinItem it;
+    uint32_t r = blockIdx.x;
+    it.split = r % p.splits; r /= p.splits;
+    const int qt = p.q_tiles - 1 - (int)(r % p.q_tiles);        // late (longer) causal tiles first
+    it.bh = r / p.q_tiles;
+    it.b = it.bh / p.heads;
+    it.h = it.bh - it.b * p.heads;
+    it.row0 = (int64_t)qt * (128 * NQ);
+    it.nq = NQ == 2 && it.row0 + 128 < p.sq ? 2 : 1;
+    it.len = keys_of(p, it.b);
+    it.offset = p.has_offset ? p.q_offset : it.len - p.sq;
+    const int64_t last = min(it.row0 + 128 * NQ, p.sq) - 1;
+    const Seen a = seen_at(p, it.row0 + it.offset, it.len), z = seen_at(p, last + it.offset, it.len);
+    // sink, lo and hi grow with the position
+    it.n1 = (z.sink + kKT - 1) / kKT;
+    it.w0 = max(it.n1, a.lo / kKT);
+    const int w1 = z.hi > a.lo ? (z.hi + kKT - 1) / kKT : 0;
+    const int total = it.n1 + max(0, w1 - it.w0);
+    it.begin = (int)((int64_t)total * it.split / p.splits);
+    it.count = (int)((int64_t)total * (it.split + 1) / p.splits) - it.begin;
+    return it;
+}
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+// D[128 x N] (+)= A B, A and B in shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+// the same with A in tensor memory
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+// 32 lanes x 32 columns from r[OFF .. OFF + 31]
+template <int OFF, int N> __device__ __forceinline__ void tmem_st32_at(uint32_t taddr, const uint32_t (&r)[N]) {
+    static_assert(OFF + 32 <= N, "range");
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+        "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(r[OFF + 0]), "r"(r[OFF + 1]), "r"(r[OFF + 2]), "r"(r[OFF + 3]), "r"(r[OFF + 4]),
+          "r"(r[OFF + 5]), "r"(r[OFF + 6]), "r"(r[OFF + 7]), "r"(r[OFF + 8]), "r"(r[OFF + 9]), "r"(r[OFF + 10]),
+          "r"(r[OFF + 11]), "r"(r[OFF + 12]), "r"(r[OFF + 13]), "r"(r[OFF + 14]), "r"(r[OFF + 15]),
+          "r"(r[OFF + 16]), "r"(r[OFF + 17]), "r"(r[OFF + 18]), "r"(r[OFF + 19]), "r"(r[OFF + 20]),
+          "r"(r[OFF + 21]), "r"(r[OFF + 22]), "r"(r[OFF + 23]), "r"(r[OFF + 24]), "r"(r[OFF + 25]),
+          "r"(r[OFF + 26]), "r"(r[OFF + 27]), "r"(r[OFF + 28]), "r"(r[OFF + 29]), "r"(r[OFF + 30]),
+          "r"(r[OFF + 31])
+        : "memory");
+}
+
+template <typename L>
+__device__ void win_producer(const WinParams& p, const WinItem& it, int fix, uint8_t* smem, const WinBars& B, volatile int* abort) {
+    prefetch_tmap(&p.tm_q);
+    prefetch_tmap(&p.tm_k);
+    prefetch_tmap(&p.tm_v);
+    mbar_arrive_expect_tx(B.q_full, it.nq * L::kBytes);
+    for (int w = 0; w < it.nq; ++w)
+        for (int x = 0; x < L::kBoxes; ++x)
+            tma_load_4d(smem + w * L::kBytes + x * L::kBox, &p.tm_q, B.q_full, 64 * x, (int)it.row0 + 128 * w, (int)it.h,
+                        (int)it.b);
+    int issued = 0;
+    for (int g = 0; g < 2 * it.count; ++g) {                     // K_0, V_0, K_1, V_1, ...
+        const int s = g % L::kStages;
+        if (g >= L::kStages && !mbar_wait(&B.kv_empty[s], ((g / L::kStages) - 1) & 1, abort)) break;
+        const int key = it.tile(g >> 1) * kKT;
+        uint64_t* bar = g == 2 * fix + 1 ? B.v_last : &B.kv_full[s];
+        mbar_arrive_expect_tx(bar, L::kBytes);
+        uint8_t* st = smem + L::kOffKV + s * L::kBytes;
+        for (int x = 0; x < L::kBoxes; ++x)
+            tma_load_4d(st + x * L::kBox, g & 1 ? &p.tm_v : &p.tm_k, bar, 64 * x, key, (int)it.h, (int)it.b);
+        issued = g + 1;
+    }
+    if (*abort) {                                                // no copy may land after the CTA exits
+        drain_wait(B.q_full, 0);
+        if (fix >= 0 && issued > 2 * fix + 1) drain_wait(B.v_last, 0);
+        for (int s = 0; s < L::kStages && s < issued; ++s)
+            drain_wait(&B.kv_full[s], ((issued - 1 - s) / L::kStages) & 1);
+    }
+}
+
+template <typename T, int HD, int NQ>
+__device__ void win_mma(const WinItem& it, uint8_t* smem, const WinBars& B, uint32_t tmem, volatile int* abort) {
+    using L = WinTile<HD, NQ>;
+    constexpr uint32_t idesc_qk = idesc_f16<T>(128, kKT), idesc_pv = idesc_f16<T>(128, HD, true);
+    const uint64_t q0 = smem_desc_k128(smem), k0 = smem_desc_k128(smem + L::kOffKV);
+    // V tile as the N-major operand: 64-channel blocks a box apart (leading
+    // offset), groups of 8 keys 1024 bytes apart (stride offset)
+    const uint64_t v0 = (k0 & ~(0x3FFFull << 16)) | ((uint64_t)(L::kBox >> 4) << 16);
+    auto qk = [&](int w, int s) {
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint32_t step = (kk / 4) * (L::kBox >> 4) + 2 * (kk % 4);
+            mma_ss(tmem + 128 * w, q0 + w * (L::kBytes >> 4) + step, k0 + s * (L::kBytes >> 4) + step, idesc_qk, kk > 0);
+        }
+    };
+    bool ok = mbar_wait(B.q_full, 0, abort) && mbar_wait(&B.kv_full[0], 0, abort);
+    if (ok) {
+        tc_fence_after();
+        for (int w = 0; w < it.nq; ++w) {
+            qk(w, 0);
+            mma_commit(&B.s_full[w]);
+        }
+        mma_commit(&B.kv_empty[0]);
+    }
+    for (int j = 0; ok && j < it.count; ++j) {
+        const int gv = 2 * j + 1, gk = 2 * j + 2;
+        const int sv = gv % L::kStages, sk = gk % L::kStages;
+        const bool more = j + 1 < it.count;
+        ok = mbar_wait(&B.kv_full[sv], (gv / L::kStages) & 1, abort);
+        for (int w = 0; ok && w < it.nq; ++w) {
+            if (!mbar_wait(&B.p_full[w], j & 1, abort)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < kKT / 16; ++kk)
+                mma_ts(tmem + L::kColO + 128 * w, tmem + 128 * w + 8 * kk, v0 + sv * (L::kBytes >> 4) + 128 * kk, idesc_pv,
+                       j > 0 || kk > 0);
+            if (w == it.nq - 1) mma_commit(&B.kv_empty[sv]);
+            if (more) {
+                if (w == 0 && !mbar_wait(&B.kv_full[sk], (gk / L::kStages) & 1, abort)) { ok = false; break; }
+                tc_fence_after();
+                qk(w, sk);
+                mma_commit(&B.s_full[w]);
+                if (w == it.nq - 1) mma_commit(&B.kv_empty[sk]);
+            } else {
+                mma_commit(&B.o_full[w]);
+            }
+        }
+    }
+    mma_commit(B.drain);
+    drain_wait(B.drain, 0);
+}
+
+// Bits [a, b) of the 32-key word that starts at key 32 w of a tile.
+__device__ __forceinline__ uint32_t bits_below(int x) { return x <= 0 ? 0u : x >= 32 ? 0xffffffffu : (1u << x) - 1u; }
+
+template <typename T, int HD, int NQ>
+__device__ void win_softmax(const WinParams& p, const WinItem& it, uint8_t* smem, const WinBars& B, uint32_t tmem, int w,
+                            int quarter, int lane, volatile int* abort) {
+    using L = WinTile<HD, NQ>;
+    const int64_t tile_row = it.row0 + 128 * w;
+    const int64_t row = tile_row + quarter * 32 + lane;
+    const bool valid = row < p.sq;
+    const bool warp_live = tile_row + quarter * 32 < p.sq;
+    const int64_t last = min(tile_row + 128, p.sq) - 1;
+    const Seen none{0, 0, 0};
+    const Seen mine = valid ? seen_at(p, row + it.offset, it.len) : none;
+    const Seen first = seen_at(p, tile_row + it.offset, it.len), end = seen_at(p, last + it.offset, it.len);
+    const uint32_t trow = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t ts = trow + 128 * w, to = trow + L::kColO + 128 * w;
+    float m = -INFINITY, den = 0.0f;
+    for (int j = 0; j < it.count; ++j) {
+        if (!mbar_wait(&B.s_full[w], j & 1, abort)) return;
+        tc_fence_after();
+        if (warp_live) {
+            uint32_t r[128];
+            tmem_ld32_at<0>(ts, r);
+            tmem_ld32_at<32>(ts + 32, r);
+            tmem_ld32_at<64>(ts + 64, r);
+            tmem_ld32_at<96>(ts + 96, r);
+            tmem_wait_ld();
+            const int k0 = it.tile(j) * kKT, k1 = k0 + kKT;
+            // all rows of the query tile see all keys of this one
+            const bool full = k1 <= first.sink || (k1 <= first.hi && (k0 >= end.lo || end.lo <= first.sink));
+            if (!full) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int o = k0 + 32 * q;
+                    const uint32_t seen = bits_below(mine.sink - o) | (bits_below(mine.hi - o) & ~bits_below(mine.lo - o));
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (!(seen & (1u << e))) r[32 * q + e] = 0xff800000u;
+                }
+            }
+            float mx[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx[e] = fmaxf(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+#pragma unroll
+            for (int t = 1; t < 8; ++t)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    mx[e] = fmax3(mx[e], __uint_as_float(r[16 * t + 2 * e]), __uint_as_float(r[16 * t + 2 * e + 1]));
+            const float top =
+                __fmul_rn(fmaxf(fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]), mx[6]), mx[7]), p.c);
+            const float m_new = top > m + 8.0f ? top : m;
+            const float alpha = m_new == m ? 1.0f : ex2_ftz(m - m_new);
+            const bool moved = __any_sync(0xffffffffu, m_new != m);
+            const float ref = m_new == -INFINITY ? 0.0f : m_new;
+            const float2 cc = make_float2(p.c, p.c), rr = make_float2(-ref, -ref);
+            uint32_t pk[64];
+#pragma unroll
+            for (int e = 0; e < 64; ++e) {
+                const float2 x = ffma2(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), cc, rr);
+                pk[e] = F16<T>::two(ex2_ftz(x.x), ex2_ftz(x.y));
+            }
+            tmem_st32_at<0>(ts, pk);
+            tmem_st32_at<32>(ts + 32, pk);
+            if (moved && j > 0) {                                // PV_w(j-1) is done: s_full follows it
+#pragma unroll 1
+                for (int q = 0; q < HD / 32; ++q) {
+                    uint32_t o[32];
+                    tmem_ld32_at<0>(to + 32 * q, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__fmul_rn(__uint_as_float(o[e]), alpha));
+                    tmem_st32_at<0>(to + 32 * q, o);
+                }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            mbar_arrive_if(&B.p_full[w], lane == 0);
+            float2 sum[4] = {};
+#pragma unroll
+            for (int e = 0; e < 64; ++e) sum[e & 3] = fadd2(sum[e & 3], F16<T>::both(pk[e]));
+            const float2 s2 = fadd2(fadd2(sum[0], sum[1]), fadd2(sum[2], sum[3]));
+            den = __fmaf_rn(den, alpha, __fadd_rn(s2.x, s2.y));
+            m = m_new;
+        } else {
+            tc_fence_before();
+            __syncwarp();
+            mbar_arrive_if(&B.p_full[w], lane == 0);
+        }
+    }
+    if (!warp_live) return;
+    if (it.count > 0) {
+        if (!mbar_wait(&B.o_full[w], 0, abort)) return;
+        tc_fence_after();
+    }
+    const bool sees = mine.sink > 0 || mine.hi > mine.lo;
+    if (p.splits > 1) {
+        const int64_t at = ((int64_t)it.split * (gridDim.x / p.splits / p.q_tiles) + it.bh) * p.sq + row;
+        if (it.count > 0) {
+            float4* dst = reinterpret_cast<float4*>(p.part + at * HD);
+#pragma unroll 1
+            for (int q = 0; q < HD / 32; ++q) {
+                uint32_t o[32];
+                tmem_ld32_at<0>(to + 32 * q, o);
+                tmem_wait_ld();
+                if (valid) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        dst[8 * q + e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                                     __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+                }
+            }
+        }
+        if (valid) p.part_ml[at] = make_float2(m, den);
+        return;
+    }
+    // out = O / den; a row that sees nothing is 0
+    const float inv = sees ? __frcp_rn(den) : 0.0f;
+    T* out = static_cast<T*>(p.out) + it.b * p.os[0] + it.h * p.os[1] + row * p.os[2];
+    bool bad = false;
+#pragma unroll 1
+    for (int q = 0; q < HD / 32; ++q) {
+        uint32_t o[32];
+        if (it.count > 0) {
+            tmem_ld32_at<0>(to + 32 * q, o);
+            tmem_wait_ld();
+        }
+        float f[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            f[e] = sees ? __fmul_rn(__uint_as_float(o[e]), inv) : 0.0f;
+            bad |= !finite_f(f[e]);
+        }
+        if (valid) {
+            if (p.vec_out) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (32 * q + 8 * e < p.d)
+                        *reinterpret_cast<uint4*>(out + 32 * q + 8 * e) =
+                            make_uint4(F16<T>::two(f[8 * e], f[8 * e + 1]), F16<T>::two(f[8 * e + 2], f[8 * e + 3]),
+                                       F16<T>::two(f[8 * e + 4], f[8 * e + 5]), F16<T>::two(f[8 * e + 6], f[8 * e + 7]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (32 * q + e < p.d) out[32 * q + e] = F16<T>::one(f[e]);
+            }
+        }
+    }
+    // rows with a NaN or infinity among the tiles' keys (or no finite logit)
+    unsigned again = __ballot_sync(0xffffffffu, valid && sees && bad);
+    if (again) {
+        float* qrow = reinterpret_cast<float*>(smem + w * L::kBytes) + 128 * quarter;    // Q_w is no longer read
+        for (; again; again &= again - 1)
+            window_row<T>(p, it.b, it.h, tile_row + quarter * 32 + __ffs(again) - 1, qrow, lane);
+    }
+}
+
+template <typename T, int HD, int NQ>
+__global__ void __launch_bounds__(WinTile<HD, NQ>::kThreads, WinTile<HD, NQ>::kCtas)
+    window_kernel(const __grid_constant__ WinParams p) {
+    pdl_wait();
+    using L = WinTile<HD, NQ>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (smem_u32(smem) & 1023u) {
+        if (threadIdx.x == 0) flag_status(p.status, VCB_FLAG_INTERNAL);
+        return;
+    }
+    const WinBars B = win_bars<L>(smem);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
+    volatile int* abort = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const WinItem it = win_item<NQ>(p);
+    if (threadIdx.x == 0) {
+        mbar_init(B.q_full, 1);
+        for (int s = 0; s < L::kStages; ++s) {
+            mbar_init(&B.kv_full[s], 1);
+            mbar_init(&B.kv_empty[s], 1);
+        }
+        for (int w = 0; w < 2; ++w) {
+            mbar_init(&B.s_full[w], 1);
+            mbar_init(&B.p_full[w], 4);
+            mbar_init(&B.o_full[w], 1);
+        }
+        mbar_init(B.v_last, 1);
+        mbar_init(B.drain, 1);
+        *abort = 0;
+        fence_barrier_init();
+    }
+    if (warp == 3) {
+        tmem_alloc(tmem_slot, L::kCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    // the place in this CTA's list of the tile that holds keys on both sides
+    // of the entry's length, when the tensor has rows there
+    int fix = -1;
+    if (it.len < p.sk && it.len % kKT && it.count > 0) {
+        const int t = (int)(it.len / kKT);
+        if (it.tile(it.count - 1) == t) fix = it.count - 1;
+    }
+    if (warp < 4) {
+        reg_dealloc<L::kRegsCtl>();
+        if (it.count > 0) {
+            if (warp == 0 && lane == 0) win_producer<L>(p, it, fix, smem, B, abort);
+            if (warp == 1 && lane == 0) win_mma<T, HD, NQ>(it, smem, B, tmem, abort);
+            if (warp == 2 && fix >= 0) {
+                const int s = (2 * fix + 1) % L::kStages;
+                if (mbar_wait(B.v_last, 0, abort)) {
+                    // whole 128-byte lines: the swizzle moves bytes within a line only
+                    const int first = (int)(it.len % kKT);
+                    for (int x = 0; x < L::kBoxes; ++x) {
+                        uint4* box = reinterpret_cast<uint4*>(smem + L::kOffKV + s * L::kBytes + x * L::kBox);
+                        for (int i = first * 8 + lane; i < kKT * 8; i += 32) box[i] = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    mbar_arrive_if(&B.kv_full[s], lane == 0);
+                }
+            }
+        }
+    } else {
+        reg_alloc<L::kRegsSoft>();
+        const int w = (warp - 4) >> 2;
+        if (w < it.nq) win_softmax<T, HD, NQ>(p, it, smem, B, tmem, w, warp & 3, lane, abort);
+    }
+    tc_fence_before();
+    __syncwarp();
+    __syncthreads();
+    if (warp == 3) {
+        tc_fence_after();
+        tmem_dealloc(tmem, L::kCols);
+    }
+    if (threadIdx.x == 0 && *abort) flag_status(p.status, VCB_FLAG_TIMEOUT);
+}
+
+// One warp per row: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) den_s over
+// the parts in order.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ WinParams p, int64_t rows) {
     pdl_wait();
     pdl_open();
     __shared__ float qrow[8][128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t i = (int64_t)blockIdx.x * 8 + warp;
-    if (i >= p.sq) return;
-    window_row<T>(p, blockIdx.y / p.heads, blockIdx.y % p.heads, i, qrow[warp], lane);
+    const int64_t r = (int64_t)blockIdx.x * 8 + warp;
+    if (r >= rows) return;
+    const int64_t bh = r / p.sq, i = r - bh * p.sq, b = bh / p.heads, h = bh - b * p.heads;
+    const int64_t len = keys_of(p, b);
+    const Seen s = seen_at(p, i + (p.has_offset ? p.q_offset : len - p.sq), len);
+    const bool sees = s.sink > 0 || s.hi > s.lo;
+    constexpr int kPer = HD / 32;                                // channels per lane
+    float acc[kPer] = {}, den = 0.0f, top = -INFINITY;
+    for (int q = 0; q < p.splits; ++q) top = fmaxf(top, p.part_ml[q * rows + r].x);
+    for (int q = 0; q < p.splits; ++q) {
+        const float2 ml = p.part_ml[q * rows + r];
+        if (ml.x == -INFINITY && ml.y == 0.0f) continue;         // no key of this part is seen
+        const float w = ex2_ftz(ml.x - top);
+        den = __fmaf_rn(ml.y, w, den);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+            acc[e] = __fmaf_rn(p.part[(q * rows + r) * HD + lane + 32 * e], w, acc[e]);
+    }
+    T* out = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + i * p.os[2];
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        const float f = sees ? __fdiv_rn(acc[e], den) : 0.0f;
+        bad |= !finite_f(f);
+        if (lane + 32 * e < p.d) out[lane + 32 * e] = F16<T>::one(f);
+    }
+    if (__any_sync(0xffffffffu, bad)) window_row<T>(p, b, h, i, qrow[warp], lane);
+}
+
+struct WinPlan {
+    int hd, nq, q_tiles, splits;
+    int pitch;                   // channels of a packed row
+    bool pack[3];                // Q, K, V
+    size_t off[3], off_part, off_ml, total;
+};
+
+WinPlan plan(const vcb_window_args* a) {
+    WinPlan r{};
+    r.hd = a->d <= 64 ? 64 : 128;
+    r.nq = a->sq <= 128 ? 1 : 2;
+    r.pitch = (a->d + 7) / 8 * 8;
+    const int64_t rows = 128 * r.nq;
+    r.q_tiles = (int)((a->sq + rows - 1) / rows);
+    const int64_t bh = a->batch * a->heads;
+    // Key tiles of a query tile (an upper bound where lengths are on the device).
+    auto tiles = [](int64_t n) { return (n + kKT - 1) / kKT; };
+    const int64_t all = tiles(a->sk);
+    int64_t right = a->causal ? 0 : a->right;
+    if (a->causal && a->right >= 0 && a->right < right) right = a->right;
+    int64_t t = all;
+    if (a->left >= 0 && right >= 0) {
+        const int64_t span = tiles(a->left + right + (a->sq < rows ? a->sq : rows)) + 1;
+        const int64_t sink = tiles(a->sinks);
+        if (sink + span < all) t = sink + span;
+    }
+    // Parts: as many as make the last wave of CTAs full, counting what a CTA
+    // spends outside its tiles (about four tiles' time) and the join.
+    const int64_t slots = (int64_t)sm_count() * (r.nq == 1 ? 2 : 1), items = bh * r.q_tiles;
+    r.splits = 1;
+    int64_t best = 0;
+    for (int64_t s = 1; s <= 32 && s <= t && items * (s - 1) < 2 * slots; ++s) {
+        const int64_t cost = (items * s + slots - 1) / slots * ((t + s - 1) / s + 4) + (s > 1 ? 4 : 0);
+        if (s == 1 || cost < best) {
+            best = cost;
+            r.splits = (int)s;
+        }
+    }
+    const void* base[3] = {a->q, a->k, a->v};
+    const int64_t* st[3] = {a->q_stride, a->k_stride, a->v_stride};
+    auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
+    size_t o = 0;
+    for (int i = 0; i < 3; ++i) {
+        const int64_t n = i ? a->sk : a->sq;
+        r.pack[i] = !on16(base[i]) || !tma_stride(st[i][0], a->batch) || !tma_stride(st[i][1], a->heads) ||
+                    !tma_stride(st[i][2], n);
+        r.off[i] = o;
+        if (r.pack[i]) o += up((size_t)(bh * n * r.pitch) * 2);
+    }
+    r.off_part = o;
+    if (r.splits > 1) o += up((size_t)(r.splits * bh * a->sq * r.hd) * 4);
+    r.off_ml = o;
+    if (r.splits > 1) o += up((size_t)(r.splits * bh * a->sq) * 8);
+    r.total = o;
+    return r;
+}
+
+template <typename T, int HD, int NQ> int launch(const WinParams& p, int64_t items, cudaStream_t st) {
+    using L = WinTile<HD, NQ>;
+    static bool ready[64] = {};
+    auto kernel = window_kernel<T, HD, NQ>;
+    int dev = 0;
+    VCB_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return fail(VCB_ERR_INVALID_ARGUMENT, "device ordinal %d out of range", dev);
+    if (!ready[dev]) {
+        VCB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem));
+        cudaFuncAttributes fa;
+        VCB_CUDA(cudaFuncGetAttributes(&fa, kernel));
+        // a setmaxnreg.inc that the launch's registers cannot serve would wait forever
+        if (fa.numRegs * L::kThreads < L::kRegSplit)
+            return fail(VCB_ERR_CUDA, "window kernel launched with %d registers x %d threads, below its %d-register split",
+                        fa.numRegs, L::kThreads, L::kRegSplit);
+        ready[dev] = true;
+    }
+    VCB_CUDA(launch_pdl(window_kernel<T, HD, NQ>, dim3((unsigned)items), dim3(L::kThreads), L::kSmem, st, p));
+    if (p.splits > 1) {
+        const int64_t rows = items / p.splits / p.q_tiles * p.sq;
+        VCB_CUDA(launch_pdl(window_join_kernel<T, HD>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p, rows));
+    }
+    return VCB_OK;
+}
+template <typename T> int launch_any(const WinParams& p, const WinPlan& r, int64_t items, cudaStream_t st) {
+    if (r.hd == 128) return r.nq == 1 ? launch<T, 128, 1>(p, items, st) : launch<T, 128, 2>(p, items, st);
+    return r.nq == 1 ? launch<T, 64, 1>(p, items, st) : launch<T, 64, 2>(p, items, st);
 }
 
 }  // namespace
 
-size_t window_workspace_bytes(const vcb_window_args*) { return 0; }
+size_t window_workspace_bytes(const vcb_window_args* a) { return plan(a).total; }
 
 int window_run(const vcb_window_args* a, cudaStream_t st) {
-    WinParams p{};
+    const WinPlan r = plan(a);
+    const int64_t bh = a->batch * a->heads, items = bh * r.q_tiles * r.splits;
+    if (items >= (1ll << 31)) return fail(VCB_ERR_INVALID_ARGUMENT, "too many query tiles for one grid");
+    WinParams p;
+    memset(&p, 0, sizeof(p));
     p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out;
     p.kv_lens = a->kv_lens;
     for (int i = 0; i < 3; ++i) {
@@ -132,10 +725,45 @@ int window_run(const vcb_window_args* a, cudaStream_t st) {
     p.left = a->left; p.right = a->right; p.sinks = a->sinks;
     p.causal = a->causal; p.has_offset = a->has_offset; p.q_offset = a->q_offset;
     p.d = a->d; p.scale = a->scale;
-    const dim3 grid((unsigned)((a->sq + 7) / 8), (unsigned)(a->batch * a->heads));
-    if (a->dtype == VCB_BF16) VCB_CUDA(launch_pdl(window_row_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p));
-    else VCB_CUDA(launch_pdl(window_row_kernel<__half>, grid, dim3(256), 0, st, p));
-    return VCB_OK;
+    p.c = (float)((double)a->scale * 1.4426950408889634);
+    p.q_tiles = r.q_tiles; p.splits = r.splits;
+    p.vec_out = on16(a->out) && by8(a->d) && by8(a->out_stride[0]) && by8(a->out_stride[1]) && by8(a->out_stride[2]);
+    char* ws = static_cast<char*>(a->workspace);
+    p.part = reinterpret_cast<float*>(ws + r.off_part);
+    p.part_ml = reinterpret_cast<float2*>(ws + r.off_ml);
+    p.status = a->status;
+    const void* base[3] = {a->q, a->k, a->v};
+    const int64_t* strides[3] = {a->q_stride, a->k_stride, a->v_stride};
+    CUtensorMap* maps[3] = {&p.tm_q, &p.tm_k, &p.tm_v};
+    PackParams pk{};
+    pk.channels = a->d;
+    pk.pitch = r.pitch;
+    int64_t blocks = 0;
+    for (int i = 0; i < 3; ++i) {
+        const int64_t n = i ? a->sk : a->sq;
+        const void* at = base[i];
+        int64_t sb = strides[i][0], sh = strides[i][1], ss = strides[i][2];
+        if (r.pack[i]) {
+            pk.side[i] = {static_cast<const uint16_t*>(at), reinterpret_cast<uint16_t*>(ws + r.off[i]), bh * n, n, sb, ss,
+                          a->heads, sh, 0, a->d};
+            blocks += (bh * n + 7) / 8;
+            at = ws + r.off[i];
+            ss = r.pitch; sh = n * ss; sb = a->heads * sh;
+        }
+        pk.end[i] = blocks;
+        // strides of axes of length one are never taken: any legal value will do
+        if (n == 1) ss = r.pitch;
+        if (a->heads == 1) sh = r.pitch;
+        if (a->batch == 1) sb = r.pitch;
+        const cuuint64_t dims[4] = {(cuuint64_t)a->d, (cuuint64_t)n, (cuuint64_t)a->heads, (cuuint64_t)a->batch};
+        const cuuint64_t bytes[3] = {(cuuint64_t)ss * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
+        const cuuint32_t box[4] = {64, 128, 1, 1};
+        int rc = make_map16(maps[i], at, a->dtype == VCB_BF16, 4, dims, bytes, box);
+        if (rc) return rc;
+    }
+    if (blocks >= (1ll << 31)) return fail(VCB_ERR_INVALID_ARGUMENT, "too many rows for one grid");
+    if (blocks) VCB_CUDA(launch_pack(pk, st));
+    return a->dtype == VCB_BF16 ? launch_any<__nv_bfloat16>(p, r, items, st) : launch_any<__half>(p, r, items, st);
 }
 
 }  // namespace vcb
