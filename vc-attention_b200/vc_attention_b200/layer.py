@@ -14,14 +14,9 @@ import math
 import torch
 
 from . import _abi
-from .b200_backend import _DTYPES, _extension, _require_b200, _stream
+from .b200_backend import _DTYPES, _extension, _require_b200
 
 ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4}
-
-
-def _rows(x):
-    """``x`` with a contiguous last axis (a copy only when it has none)."""
-    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
 
 
 def _interval(t):
@@ -71,6 +66,64 @@ def _same_view(a, b):
     return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype
 
 
+# A call's checks and argument struct depend on its tensors' shapes, strides,
+# types and devices and on its options alone.  They are worked out once for each
+# such combination; a call then only fills in the addresses.  (Checking anew
+# took 20-30 us of host time a call, more than the small calls take on the GPU.)
+_PLANS = {}
+
+
+def _meta(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _remember(key, plan):
+    if len(_PLANS) >= 1024:
+        _PLANS.clear()
+    _PLANS[key] = plan
+    return plan
+
+
+class _Plan:
+    """Arguments without addresses (``args``), the scratch bytes for 16-byte
+    aligned operands (``need``), the C entry points, and the operands that have
+    no contiguous last axis (``copy``)."""
+
+    def __init__(self, args, entry, copy=(), workspace=None, operands=()):
+        lib = _extension()
+        self.lib, self.entry, self.copy, self.operands = lib, getattr(lib, entry), copy, operands
+        self.workspace = None if workspace is None else getattr(lib, workspace)
+        self.cls, self.need = type(args), 0
+        if workspace is not None and not copy:
+            for name in operands:
+                setattr(args, name, 256)
+            self.need = self.workspace(ctypes.byref(args))
+        self.args = bytes(args)
+
+    def call(self, device, **pointers):
+        a = self.cls.from_buffer_copy(self.args)
+        for name, value in pointers.items():
+            setattr(a, name, value)
+        need = self.need
+        if self.workspace is not None and any(pointers[name] & 15 for name in self.operands):
+            need = self.workspace(ctypes.byref(a))
+        if need:
+            scratch = torch.empty(need, dtype=torch.uint8, device=device)
+            a.workspace, a.workspace_bytes = scratch.data_ptr(), need
+        stream = torch._C._cuda_getCurrentRawStream(device.index)      # current_stream() makes an object: 3 us
+        if torch.cuda.current_device() == device.index:
+            rc = self.entry(ctypes.byref(a), stream)
+        else:
+            with torch.cuda.device(device):
+                rc = self.entry(ctypes.byref(a), stream)
+        if rc:
+            _abi.check(self.lib, rc)
+
+
+def _no_rows(t):
+    return t is not None and t.shape[-1] != 1 and t.stride(-1) != 1
+
+
 def _check_out(out, shape, like, what, inputs, may_be=None):
     """An output the caller gives: shape, type, device, a contiguous last axis,
     no overlap with itself or with an input other than ``may_be`` itself."""
@@ -102,7 +155,6 @@ def _side_dtype(t, like, what):
     return _DTYPES[t.dtype]
 
 
-@torch.no_grad()
 def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, heads_in=False, heads_out=None,
            out=None, status=None):
     """``residual + gate * act(x @ weight.T + bias)`` in one kernel.
@@ -120,10 +172,32 @@ def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, h
     given, with any strides but a contiguous last axis; it may be ``residual``
     itself and shares memory with no other input.
 
-    The call only queues work on the current stream.  ``status``: a
-    caller-owned, zeroed one-element int32 CUDA tensor that receives the
-    kernel's flags for ``b200_backend.raise_for_status`` (an expired device
-    wait)."""
+    The call only queues work on the current stream, and its result carries no
+    gradient.  ``status``: a caller-owned, zeroed one-element int32 CUDA tensor
+    that receives the kernel's flags for ``b200_backend.raise_for_status`` (an
+    expired device wait)."""
+    key = ("linear", _meta(x), _meta(weight), _meta(bias), activation, _meta(gate), _meta(residual), bool(heads_in),
+           heads_out, type(heads_out), _meta(out), _meta(status))
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = _linear_plan(x, weight, bias, activation, gate, residual, bool(heads_in), heads_out, out, status)
+        _remember(key, plan)
+    if out is not None:
+        _check_out(out, plan.shape, x, "out", (x, weight, bias, gate, residual), may_be=residual)
+    if plan.copy:
+        x, weight, bias, gate, residual = (t.contiguous() if _no_rows(t) else t
+                                           for t in (x, weight, bias, gate, residual))
+        return linear(x, weight, bias, activation=activation, gate=gate, residual=residual, heads_in=heads_in,
+                      heads_out=heads_out, out=out, status=status)
+    if out is None:
+        out = torch.empty(plan.shape, dtype=x.dtype, device=x.device)
+    plan.call(x.device, x=x.data_ptr(), w=weight.data_ptr(), y=out.data_ptr(), bias=_ptr(bias), gate=_ptr(gate),
+              residual=_ptr(residual), status=_ptr(status))
+    return out
+
+
+def _linear_plan(x, weight, bias, activation, gate, residual, heads_in, heads_out, out, status):
+    """The checks of ``linear`` and its arguments without addresses."""
     if activation not in ACTIVATIONS:
         raise ValueError('activation must be None, "silu", "gelu", "gelu_tanh" or "relu"')
     if x.dtype not in (torch.float16, torch.bfloat16):
@@ -154,17 +228,15 @@ def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, h
         shape = (b, heads_out, s, n // heads_out)
     else:
         shape = (*lead, n)
-    if bias is not None:
-        if tuple(bias.shape) != (n,):
-            raise ValueError(f"bias must be [{n}]")
-        bias_dtype = _side_dtype(bias, x, "bias")
-        bias = bias.contiguous()
+    if bias is not None and tuple(bias.shape) != (n,):
+        raise ValueError(f"bias must be [{n}]")
+    bias_dtype = 0 if bias is None else _side_dtype(bias, x, "bias")
+    gate_dtype = 0
     if gate is not None:
         gate_dtype = _side_dtype(gate, x, "gate")
         if gate.ndim < 1 or gate.ndim > len(shape) or gate.shape[-1] != n or any(
                 g not in (1, full) for g, full in zip(reversed(gate.shape), reversed(shape))):
             raise ValueError(f"gate must broadcast against {shape} with its last axis of {n}")
-        gate = _rows(gate).expand(b, s, n)
     if residual is not None and (tuple(residual.shape) != shape or residual.dtype != x.dtype or
                                  residual.device != x.device):
         raise ValueError("residual must have the result's shape, dtype and device")
@@ -172,41 +244,30 @@ def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, h
     if out is not None:
         _check_out(out, shape, x, "out", (x, weight, bias, gate, residual), may_be=residual)
     _require_b200(x, "linear")
-    lib = _extension()
-    x, weight = _rows(x), _rows(weight)
-    if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    res = None if residual is None else _rows(residual)
+    copy = tuple(i for i, t in enumerate((x, weight, bias, gate, residual)) if _no_rows(t))
     if heads_in:
-        xs = (x.stride(0), x.stride(1), x.stride(2))
+        xs = x.stride()[:3]
     else:
         xs = (x.stride(0) if x.ndim == 3 else 0, 0, x.stride(-2))
+    n_head = n if heads_out is None else n // heads_out
     if heads_out is not None:
-        n_head, ys = n // heads_out, out.stride()[:3]
+        ys = (heads_out * s * n_head, s * n_head, n_head) if out is None else out.stride()[:3]
+    elif out is None:
+        ys = (s * n, 0, n)
     else:
-        n_head, ys = n, (out.stride(0) if out.ndim == 3 else 0, 0, out.stride(-2))
-    a = _abi.LinearArgs(
-        x=x.data_ptr(), w=weight.data_ptr(), dtype=_DTYPES[x.dtype], batch=b, tokens=s, n=n, heads_in=hi, k_head=kh,
-        x_stride_b=xs[0], x_stride_h=xs[1], x_stride_s=xs[2], w_stride=weight.stride(0) if n > 1 else k,
-        activation=ACTIVATIONS[activation], y=out.data_ptr(), n_head=n_head, y_stride_b=ys[0], y_stride_h=ys[1],
-        y_stride_s=ys[2], status=_ptr(status))
-    if bias is not None:
-        a.bias, a.bias_dtype = bias.data_ptr(), bias_dtype
-    if gate is not None:
-        a.gate, a.gate_dtype, a.gate_stride_b, a.gate_stride_s = gate.data_ptr(), gate_dtype, *gate.stride()[:2]
-    if res is not None:
-        a.residual = res.data_ptr()
-        a.residual_stride_b, a.residual_stride_s = (res.stride(0) if res.ndim == 3 else 0), res.stride(-2)
-    need = lib.vcb_linear_workspace(ctypes.byref(a))
-    if need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), need
-    with torch.cuda.device(x.device):
-        _abi.check(lib, lib.vcb_linear(ctypes.byref(a), _stream(x.device)))
-    return out
+        ys = (out.stride(0) if out.ndim == 3 else 0, 0, out.stride(-2))
+    gs = gate.expand(b, s, n).stride() if gate is not None else (0, 0)
+    rs = (0, 0) if residual is None else (residual.stride(0) if residual.ndim == 3 else 0, residual.stride(-2))
+    plan = _Plan(_abi.LinearArgs(
+        dtype=_DTYPES[x.dtype], batch=b, tokens=s, n=n, heads_in=hi, k_head=kh, x_stride_b=xs[0], x_stride_h=xs[1],
+        x_stride_s=xs[2], w_stride=weight.stride(0) if n > 1 else k, bias_dtype=bias_dtype,
+        activation=ACTIVATIONS[activation], gate_dtype=gate_dtype, gate_stride_b=gs[0], gate_stride_s=gs[1],
+        residual_stride_b=rs[0], residual_stride_s=rs[1], n_head=n_head, y_stride_b=ys[0], y_stride_h=ys[1],
+        y_stride_s=ys[2]), "vcb_linear", copy, "vcb_linear_workspace", ("x", "w"))
+    plan.shape = shape
+    return plan
 
 
-@torch.no_grad()
 def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, *, eps=1e-6, interleaved=True, out=None):
     """RMS norm of each head's row of Q and K and the position rotation, in
     one pass: ``n = x / sqrt(mean(x^2) + eps) * weight`` over the head's
@@ -224,7 +285,50 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, *, eps=
 
     Returns (q, k) as contiguous BNSD tensors, or writes ``out=(q_out,
     k_out)``, for example rows of a K buffer; an output may be its own
-    input."""
+    input.  The call only queues work on the current stream, and its results
+    carry no gradient."""
+    if out is None:
+        outs = None
+    else:
+        if len(out) != 2:
+            raise ValueError("out must be (q_out, k_out)")
+        outs = _meta(out[0]), _meta(out[1])
+    key = ("rope", _meta(q), _meta(k), _meta(q_weight), _meta(k_weight), _meta(cos), _meta(sin), eps, bool(interleaved),
+           outs)
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = _remember(key, _rope_plan(q, k, q_weight, k_weight, cos, sin, eps, bool(interleaved), out))
+    if out is not None:
+        _check_rope_out(out, q, k, q_weight, k_weight, cos, sin)
+    if plan.copy:
+        if cos is not None and cos.stride() != sin.stride():
+            cos, sin = cos.contiguous(), sin.contiguous()
+        q, k, q_weight, k_weight, cos, sin = (t.contiguous() if _no_rows(t) else t
+                                              for t in (q, k, q_weight, k_weight, cos, sin))
+        return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps=eps, interleaved=interleaved, out=out)
+    if out is None:
+        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    else:
+        qo, ko = out
+    plan.call(q.device, q=q.data_ptr(), k=k.data_ptr(), q_out=qo.data_ptr(), k_out=ko.data_ptr(),
+              q_weight=_ptr(q_weight), k_weight=_ptr(k_weight), cos=_ptr(cos), sin=_ptr(sin))
+    return qo, ko
+
+
+def _check_rope_out(out, q, k, *others):
+    _check_out(out[0], q.shape, q, "q_out", (q, k, *others), may_be=q)
+    _check_out(out[1], k.shape, k, "k_out", (k, q, *others), may_be=k)
+    if _shares_memory(out[0], out[1]):
+        raise ValueError("q_out and k_out must not share memory")
+
+
+def _packed_strides(shape):
+    return tuple(math.prod(shape[i + 1:]) for i in range(3))
+
+
+def _rope_plan(q, k, q_weight, k_weight, cos, sin, eps, interleaved, out):
+    """The checks of ``qk_norm_rope`` and its arguments without addresses."""
     for name, t in (("q", q), ("k", k)):
         if t.ndim != 4 or 0 in t.shape:
             raise ValueError(f"{name} must be a nonempty [B, H, S, D] tensor")
@@ -247,6 +351,8 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, *, eps=
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
     rows = rotary = 0
+    ts = (0, 0)
+    copy = tuple(i for i, t in enumerate((q, k, q_weight, k_weight, cos, sin)) if _no_rows(t))
     if cos is not None:
         if cos.shape != sin.shape or cos.ndim not in (2, 3) or 0 in cos.shape:
             raise ValueError("cos and sin must be nonempty [R, r / 2] or [B, R, r / 2] tables of one shape")
@@ -259,33 +365,18 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, *, eps=
             raise ValueError("the tables rotate more channels than a head has")
         if cos.ndim == 3 and cos.shape[0] not in (1, b):
             raise ValueError("batched tables need one entry, or one for each batch entry")
-        cos, sin = _rows(cos), _rows(sin)
         if cos.stride() != sin.stride():
-            cos, sin = cos.contiguous(), sin.contiguous()
+            copy = (*copy, 4, 5)
+        ts = (cos.stride(0) if cos.ndim == 3 and cos.shape[0] > 1 else 0, cos.stride(-2))
     if out is not None:
-        if len(out) != 2:
-            raise ValueError("out must be (q_out, k_out)")
-        others = (q_weight, k_weight, cos, sin)
-        _check_out(out[0], q.shape, q, "q_out", (q, k, *others), may_be=q)
-        _check_out(out[1], k.shape, k, "k_out", (k, q, *others), may_be=k)
-        if _shares_memory(out[0], out[1]):
-            raise ValueError("q_out and k_out must not share memory")
+        _check_rope_out(out, q, k, q_weight, k_weight, cos, sin)
     _require_b200(q, "qk_norm_rope")
-    lib = _extension()
-    q, k = _rows(q), _rows(k)
-    qo, ko = out if out is not None else (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-    q_weight, k_weight = (None if t is None else t.contiguous() for t in (q_weight, k_weight))
+    qs, ks = (_packed_strides(t.shape) if out is None else o.stride()[:3]
+              for t, o in ((q, out and out[0]), (k, out and out[1])))
     triple = ctypes.c_int64 * 3
-    a = _abi.QKNormRopeArgs(
-        q=q.data_ptr(), k=k.data_ptr(), q_out=qo.data_ptr(), k_out=ko.data_ptr(), dtype=_DTYPES[q.dtype], batch=b,
-        q_heads=h, k_heads=k.shape[1], tokens=s, d=d, q_stride=triple(*q.stride()[:3]),
-        k_stride=triple(*k.stride()[:3]), q_out_stride=triple(*qo.stride()[:3]),
-        k_out_stride=triple(*ko.stride()[:3]), q_weight=_ptr(q_weight), k_weight=_ptr(k_weight),
-        weight_dtype=_DTYPES[weights[0].dtype] if weights else 0, rows=rows, rotary=rotary,
-        interleaved=int(bool(interleaved)), norm=int(eps is not None), eps=0.0 if eps is None else float(eps))
-    if cos is not None:
-        a.cos, a.sin, a.table_stride_s = cos.data_ptr(), sin.data_ptr(), cos.stride(-2)
-        a.table_stride_b = cos.stride(0) if cos.ndim == 3 and cos.shape[0] > 1 else 0
-    with torch.cuda.device(q.device):
-        _abi.check(lib, lib.vcb_qk_norm_rope(ctypes.byref(a), _stream(q.device)))
-    return qo, ko
+    return _Plan(_abi.QKNormRopeArgs(
+        dtype=_DTYPES[q.dtype], batch=b, q_heads=h, k_heads=k.shape[1], tokens=s, d=d, q_stride=triple(*q.stride()[:3]),
+        k_stride=triple(*k.stride()[:3]), q_out_stride=triple(*qs), k_out_stride=triple(*ks),
+        weight_dtype=_DTYPES[weights[0].dtype] if weights else 0, rows=rows, rotary=rotary, table_stride_b=ts[0],
+        table_stride_s=ts[1], interleaved=int(interleaved), norm=int(eps is not None),
+        eps=0.0 if eps is None else float(eps)), "vcb_qk_norm_rope", copy)

@@ -12,8 +12,8 @@ import math
 import torch
 
 from . import _abi
-from .b200_backend import _DTYPES, _extension, _require_b200, _stream
-from .layer import _check_out, _check_status, _ptr, _rows
+from .b200_backend import _DTYPES, _require_b200
+from .layer import _PLANS, _Plan, _check_out, _check_status, _meta, _no_rows, _packed_strides, _ptr, _remember
 
 
 def _bound(value, name):
@@ -24,7 +24,6 @@ def _bound(value, name):
     return min(value, 1 << 39)
 
 
-@torch.no_grad()
 def window_attention(q, k, v, *, window=(None, None), sinks=0, causal=False, q_offset=None, kv_lens=None, scale=None,
                      out=None, status=None):
     """softmax(scale * q @ k.T) @ v over the keys that each query sees.
@@ -40,7 +39,30 @@ def window_attention(q, k, v, *, window=(None, None), sinks=0, causal=False, q_o
     ``scale`` defaults to D ** -0.5.
 
     Returns [B, H, Sq, D], or writes ``out``, which shares no memory with an
-    input.  The call only queues work; ``status`` is as for ``linear``."""
+    input.  The call only queues work on the current stream, and its result
+    carries no gradient; ``status`` is as for ``linear``."""
+    if len(window) != 2:
+        raise ValueError("window must be (left, right)")
+    key = ("window", _meta(q), _meta(k), _meta(v), *window, *(type(w) for w in window), sinks, type(sinks), bool(causal),
+           q_offset, type(q_offset), _meta(kv_lens), scale, _meta(out), _meta(status))
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = _remember(key, _window_plan(q, k, v, window, sinks, bool(causal), q_offset, kv_lens, scale, out, status))
+    if out is not None:
+        _check_out(out, q.shape, q, "out", (q, k, v, kv_lens))
+    if plan.copy:
+        q, k, v, kv_lens = (t.contiguous() if _no_rows(t) else t for t in (q, k, v, kv_lens))
+        return window_attention(q, k, v, window=window, sinks=sinks, causal=causal, q_offset=q_offset, kv_lens=kv_lens,
+                                scale=scale, out=out, status=status)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    plan.call(q.device, q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), kv_lens=_ptr(kv_lens),
+              status=_ptr(status))
+    return out
+
+
+def _window_plan(q, k, v, window, sinks, causal, q_offset, kv_lens, scale, out, status):
+    """The checks of ``window_attention`` and its arguments without addresses."""
     if any(t.ndim != 4 for t in (q, k, v)):
         raise ValueError("Expected BNSD tensors")
     if q.shape[:2] != k.shape[:2] or k.shape != v.shape or q.shape[3] != k.shape[3]:
@@ -54,8 +76,6 @@ def window_attention(q, k, v, *, window=(None, None), sinks=0, causal=False, q_o
     b, h, sq, d = q.shape
     if d > 128:
         raise ValueError("window_attention supports head dimensions <= 128")
-    if len(window) != 2:
-        raise ValueError("window must be (left, right)")
     left, right = _bound(window[0], "left"), _bound(window[1], "right")
     if sinks is None:
         raise ValueError("sinks must be a non-negative integer")
@@ -67,29 +87,17 @@ def window_attention(q, k, v, *, window=(None, None), sinks=0, causal=False, q_o
                                 kv_lens.device != q.device):
         raise ValueError("kv_lens must be an int32 tensor [B] on the inputs' device")
     scale = d ** -0.5 if scale is None else scale
-    if not math.isfinite(scale) or scale <= 0:
-        raise ValueError("scale must be positive and finite")
+    if not math.isfinite(scale) or not 1e-30 <= scale <= 1e30:
+        raise ValueError("scale must be positive and finite, in [1e-30, 1e30]")
     _check_status(status, q.device)
     if out is not None:
         _check_out(out, q.shape, q, "out", (q, k, v, kv_lens))
     _require_b200(q, "window_attention")
-    lib = _extension()
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if kv_lens is not None:
-        kv_lens = kv_lens.contiguous()
     triple = ctypes.c_int64 * 3
-    a = _abi.WindowArgs(
-        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), dtype=_DTYPES[q.dtype], batch=b, heads=h,
-        sq=sq, sk=k.shape[2], d=d, q_stride=triple(*q.stride()[:3]), k_stride=triple(*k.stride()[:3]),
-        v_stride=triple(*v.stride()[:3]), out_stride=triple(*out.stride()[:3]), kv_lens=_ptr(kv_lens), left=left,
-        right=right, sinks=first, causal=int(bool(causal)), has_offset=int(q_offset is not None),
-        q_offset=q_offset or 0, scale=float(scale), status=_ptr(status))
-    need = lib.vcb_window_workspace(ctypes.byref(a))
-    if need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), need
-    with torch.cuda.device(q.device):
-        _abi.check(lib, lib.vcb_window_attention(ctypes.byref(a), _stream(q.device)))
-    return out
+    return _Plan(_abi.WindowArgs(
+        dtype=_DTYPES[q.dtype], batch=b, heads=h, sq=sq, sk=k.shape[2], d=d, q_stride=triple(*q.stride()[:3]),
+        k_stride=triple(*k.stride()[:3]), v_stride=triple(*v.stride()[:3]),
+        out_stride=triple(*(_packed_strides(q.shape) if out is None else out.stride()[:3])), left=left, right=right,
+        sinks=first, causal=int(causal), has_offset=int(q_offset is not None), q_offset=q_offset or 0,
+        scale=float(scale)), "vcb_window_attention", tuple(i for i, t in enumerate((q, k, v, kv_lens)) if _no_rows(t)),
+        "vcb_window_workspace", ("q", "k", "v"))
