@@ -77,7 +77,9 @@ LINEAR = [
     (1, 1, 8, 8), (1, 1, 128, 64), (1, 1, 5120, 520), (2, 1, 1000, 24), (1, 2, 64, 16), (3, 5, 72, 40),
     (1, 16, 512, 4096), (1, 17, 136, 264), (1, 100, 520, 1032), (1, 127, 256, 256), (1, 128, 64, 256),
     (1, 129, 320, 248), (2, 255, 192, 504), (1, 257, 1024, 768), (1, 600, 128, 2048), (3, 333, 640, 1304),
-    (1, 2100, 264, 4104),
+    (1, 2100, 264, 4104), (1, 32, 640, 96), (4, 8, 1032, 72), (1, 33, 640, 96), (5, 7, 2048, 136),
+    # tiles cut along K, alone and behind whole ones
+    (1, 64, 5120, 512), (2, 200, 4096, 1000), (1, 2600, 2048, 2048),
     # off the 16-byte grid
     (1, 1, 1, 1), (1, 1, 77, 33), (1, 7, 9, 5), (2, 33, 100, 65), (1, 130, 257, 255), (3, 257, 1147, 2049),
 ]

@@ -26,6 +26,15 @@
 // hold 32 consecutive columns of a row: bias, gate and residual are read and y
 // written in 64-byte runs.
 //
+// Tiles that do not fill the last round of pairs are cut along K: their 64-channel
+// chunks are dealt evenly to all pairs (LinWork), a piece that is not a whole
+// tile goes to the workspace in FP32, and linear_join_kernel adds a tile's
+// pieces in order and runs the epilogue.
+//
+// Up to 32 rows the product is a stream over w: linear_few_kernel reads w
+// straight into mma.sync fragments (tcgen05 would spend its 128-row tile on
+// them), 16 or 32 rows of w per CTA, K dealt to its eight warps.
+//
 // Operands that TMA cannot address (rows or bases off the 16-byte grid) are
 // first copied, padded, into the caller's workspace.
 //
@@ -66,6 +75,9 @@ struct LinParams {
     int64_t tokens;
     int collapsed;               // rows run over batch x tokens
     int n, n_head;
+    int dp_tiles;                // tiles walked whole; the rest is cut along K
+    int cut_units, cut_each;     // chunks of the cut tiles, and of one pair's share
+    float* part;                 // [2 per pair][256][BN]
     int activation;
     const void* bias;
     const void* gate;
@@ -116,6 +128,32 @@ __device__ __forceinline__ void tile_at(const LinParams& p, int t, int& m, int& 
     m = first + (r - n * size);
 }
 
+// The i-th piece of work of pair c: a tile and its chunks [k0, k1); slot < 0
+// for a whole tile, else its place among the partial sums.  First every
+// ncl-th whole tile, then the pair's share of the cut tiles, which covers the
+// end of one tile, whole tiles and the beginning of another: two slots suffice.
+struct LinWork {
+    int tile, k0, k1, slot;
+    __device__ __forceinline__ bool get(const LinParams& p, int c, int ncl, int i) {
+        const int whole = local_items(p.dp_tiles, c, ncl);
+        if (i < whole) {
+            tile = c + i * ncl;
+            k0 = 0; k1 = p.k_chunks; slot = -1;
+            return true;
+        }
+        const int64_t a64 = (int64_t)c * p.cut_each;
+        if (a64 >= p.cut_units) return false;
+        const int a = (int)a64, b = min(p.cut_units - a, p.cut_each) + a;
+        const int t = a / p.k_chunks + i - whole;
+        const int begin = max(a, t * p.k_chunks), end = min(b, (t + 1) * p.k_chunks);
+        if (begin >= end) return false;
+        tile = p.dp_tiles + t;
+        k0 = begin - t * p.k_chunks; k1 = end - t * p.k_chunks;
+        slot = k1 - k0 == p.k_chunks ? -1 : 2 * c + (begin == a ? 0 : 1);
+        return true;
+    }
+};
+
 template <int BN>
 __device__ void lin_producer(const LinParams& p, uint8_t* smem, const LinBars& B, const Waiter& wait, uint32_t rank,
                              int c, int ncl) {
@@ -125,17 +163,17 @@ __device__ void lin_producer(const LinParams& p, uint8_t* smem, const LinBars& B
     const uint32_t lead = peer_addr(B.full, 0);
     uint32_t g = 0;
     bool ok = true;
-    const int tiles = p.m_tiles * p.n_tiles;
-    for (int t = c; ok && t < tiles; t += ncl) {
+    LinWork wk;
+    for (int i = 0; ok && wk.get(p, c, ncl, i); ++i) {
         int mt, nt;
-        tile_at(p, t, mt, nt);
+        tile_at(p, wk.tile, mt, nt);
         const int b = mt / p.m_tiles_per_batch;
         const int row = (mt - b * p.m_tiles_per_batch) * 256 + (int)rank * 128;
         const int wrow = nt * BN + (int)rank * (BN / 2);
-        int head = 0, x = 0;
-        for (int k = 0; k < p.k_chunks; ++k, ++g) {
+        int head = wk.k0 / p.chunks_per_head, x = (wk.k0 - head * p.chunks_per_head) * kBK;
+        for (int k = wk.k0; k < wk.k1; ++k, ++g) {
             const int s = g % L::kStages;
-            if (g >= (uint32_t)L::kStages && !wait(&B.empty[s], ((g / L::kStages) - 1) & 1)) {
+            if (g >= (uint32_t)L::kStages && !wait.parked(&B.empty[s], ((g / L::kStages) - 1) & 1)) {
                 ok = false;
                 break;
             }
@@ -168,15 +206,15 @@ __device__ void lin_mma(const LinParams& p, uint8_t* smem, const LinBars& B, con
     constexpr uint32_t idesc = idesc_f16<T>(256, BN);
     const uint64_t d64 = smem_desc_k128(smem);
     const uint32_t hi = (uint32_t)(d64 >> 32), lo0 = (uint32_t)d64;
-    const int tiles = p.m_tiles * p.n_tiles;
-    uint32_t g = 0, li = 0;
+    uint32_t g = 0;
     bool ok = true;
-    for (int t = c; ok && t < tiles; t += ncl, ++li) {
-        const uint32_t buf = li & 1;
-        if (li >= 2 && !wait(&B.acc_free[buf], ((li - 2) >> 1) & 1)) break;
+    LinWork wk;
+    for (int i = 0; ok && wk.get(p, c, ncl, i); ++i) {
+        const uint32_t buf = i & 1;
+        if (i >= 2 && !wait(&B.acc_free[buf], ((i - 2) >> 1) & 1)) break;
         tc_fence_after();
         const uint32_t d = tmem + buf * BN;
-        for (int k = 0; k < p.k_chunks; ++k, ++g) {
+        for (int k = wk.k0; k < wk.k1; ++k, ++g) {
             const uint32_t s = g % L::kStages;
             if (!wait(&B.full[s], (g / L::kStages) & 1)) {
                 ok = false;
@@ -185,7 +223,7 @@ __device__ void lin_mma(const LinParams& p, uint8_t* smem, const LinBars& B, con
             tc_fence_after();
             const uint32_t a = lo0 + s * (L::kStageBytes >> 4), w = a + (kABytes >> 4);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) mma2_f16(d, a + 2 * kk, w + 2 * kk, hi, idesc, k > 0 || kk > 0);
+            for (int kk = 0; kk < 4; ++kk) mma2_f16(d, a + 2 * kk, w + 2 * kk, hi, idesc, k > wk.k0 || kk > 0);
             commit_both(&B.empty[s]);
         }
         if (ok) commit_both(&B.acc_full[buf]);
@@ -242,11 +280,24 @@ __device__ __forceinline__ void load8_any(const void* p, int64_t i, int dtype, i
     }
 }
 
+// Where a row's output, gate and residual begin.
+struct RowAt {
+    int64_t y, g, r;
+    bool live;
+};
+__device__ __forceinline__ RowAt row_at(const LinParams& p, int64_t b, int64_t row) {
+    int64_t s = row;
+    if (p.collapsed) {
+        b = (uint32_t)row / (uint32_t)p.tokens;
+        s = row - b * p.tokens;
+    }
+    return {b * p.ys_b + s * p.ys_s, b * p.gs_b + s * p.gs_s, b * p.rs_b + s * p.rs_s, row < p.rows};
+}
+
 // Eight accumulated columns n .. n + 7 of one row: act, gate, residual, store.
 // f holds the sums with the bias added.
 template <typename T>
-__device__ __forceinline__ void finish8(const LinParams& p, float* f, int n, int64_t y_off, int64_t g_off,
-                                        int64_t r_off) {
+__device__ __forceinline__ void finish8(const LinParams& p, float* f, int n, const RowAt& at) {
     const int valid = p.n - n;
     if (p.activation != VCB_ACT_NONE) {
 #pragma unroll
@@ -254,17 +305,17 @@ __device__ __forceinline__ void finish8(const LinParams& p, float* f, int n, int
     }
     if (p.gate) {
         float q[8];
-        load8_any(p.gate, g_off + n, p.gate_dtype, valid, p.vec_gate, q);
+        load8_any(p.gate, at.g + n, p.gate_dtype, valid, p.vec_gate, q);
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(f[e], q[e]);
     }
     if (p.residual) {
         float q[8];
-        load8_any(p.residual, r_off + n, F16<T>::kDtype, valid, p.vec_r, q);
+        load8_any(p.residual, at.r + n, F16<T>::kDtype, valid, p.vec_r, q);
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = __fadd_rn(f[e], q[e]);
     }
-    T* y = static_cast<T*>(p.y) + y_off;
+    T* y = static_cast<T*>(p.y) + at.y;
     if (p.vec_y && valid >= 8) {
         const int h = n / p.n_head;
         *reinterpret_cast<uint4*>(y + h * p.ys_h + (n - h * p.n_head)) =
@@ -290,30 +341,20 @@ __device__ void lin_epilogue(const LinParams& p, uint8_t* smem, const LinBars& B
     float4* stage = reinterpret_cast<float4*>(smem + L::kOffEpi + ew * kEpiBytes);
     const uint32_t trow = tmem + ((uint32_t)(quarter * 32) << 16) + side * kHalfCols;
     const int r0 = lane >> 2, q8 = (lane & 3) * 8;      // this lane's first row and columns in a block
-    const int tiles = p.m_tiles * p.n_tiles;
-    uint32_t li = 0;
-    for (int t = c; t < tiles; t += ncl, ++li) {
+    LinWork wk;
+    for (int li = 0; wk.get(p, c, ncl, li); ++li) {
         int mt, nt;
-        tile_at(p, t, mt, nt);
+        tile_at(p, wk.tile, mt, nt);
         const int tb = mt / p.m_tiles_per_batch;
         const int64_t row0 = (int64_t)(mt - tb * p.m_tiles_per_batch) * 256 + rank * 128 + quarter * 32 + r0;
-        int64_t y_off[4], g_off[4], r_off[4];
-        bool live[4];
+        RowAt at[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t row = row0 + 8 * i;
-            live[i] = row < p.rows;
-            int64_t b = tb, s = row;
-            if (p.collapsed) {
-                b = p.rows < (1ll << 31) ? (int64_t)((uint32_t)row / (uint32_t)p.tokens) : row / p.tokens;
-                s = row - b * p.tokens;
-            }
-            y_off[i] = b * p.ys_b + s * p.ys_s;
-            g_off[i] = b * p.gs_b + s * p.gs_s;
-            r_off[i] = b * p.rs_b + s * p.rs_s;
-        }
+        for (int i = 0; i < 4; ++i) at[i] = row_at(p, tb, row0 + 8 * i);
+        float* part = wk.slot < 0 ? nullptr
+                                  : p.part + ((int64_t)wk.slot * 256 + rank * 128 + quarter * 32 + r0) * BN +
+                                        side * kHalfCols + q8;
         const uint32_t buf = li & 1;
-        if (!wait(&B.acc_full[buf], (li >> 1) & 1)) return;
+        if (!wait.parked(&B.acc_full[buf], (li >> 1) & 1)) return;
         tc_fence_after();
 #pragma unroll 1
         for (int ch = 0; ch < kChunks; ++ch) {
@@ -334,18 +375,25 @@ __device__ void lin_epilogue(const LinParams& p, uint8_t* smem, const LinBars& B
             const int n = nt * BN + side * kHalfCols + ch * 32 + q8;
             if (n < p.n) {
                 float bias[8];
-                if (p.bias) load8_any(p.bias, n, p.bias_dtype, p.n - n, p.vec_bias, bias);
+                if (p.bias && !part) load8_any(p.bias, n, p.bias_dtype, p.n - n, p.vec_bias, bias);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int row = r0 + 8 * i;
                     const float4 a = stage[row * 8 + ((q8 >> 2) ^ (row & 7))];
                     const float4 d = stage[row * 8 + (((q8 >> 2) + 1) ^ (row & 7))];
+                    if (!at[i].live) continue;
+                    if (part) {
+                        float4* to = reinterpret_cast<float4*>(part + (int64_t)(8 * i) * BN + ch * 32);
+                        to[0] = a;
+                        to[1] = d;
+                        continue;
+                    }
                     float f[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
                     if (p.bias) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) f[e] = __fadd_rn(f[e], bias[e]);
                     }
-                    if (live[i]) finish8<T>(p, f, n, y_off[i], g_off[i], r_off[i]);
+                    finish8<T>(p, f, n, at[i]);
                 }
             }
             __syncwarp();
@@ -409,9 +457,173 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_kernel(const __grid_con
     if (threadIdx.x == 0 && *abort) flag_status(p.status, VCB_FLAG_TIMEOUT);
 }
 
+// A cut tile's pieces, added in the order of their chunks, then the epilogue;
+// one thread per row and eight columns.
 template <typename T, int BN>
-int launch_tiles(LinParams& p, cudaStream_t st) {
-    static int max_pairs[64] = {};
+__global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ LinParams p) {
+    pdl_wait();
+    pdl_open();
+    constexpr int kGroups = BN / 8, kRowsPer = 256 / kGroups;
+    const int t = blockIdx.x / (256 / kRowsPer);             // cut tile
+    const int row = (blockIdx.x % (256 / kRowsPer)) * kRowsPer + threadIdx.x / kGroups;
+    const int col = threadIdx.x % kGroups * 8;
+    const int first = t * p.k_chunks, last = first + p.k_chunks - 1;
+    const int c0 = first / p.cut_each, c1 = last / p.cut_each;
+    if (c0 == c1) return;                                     // one pair had the whole tile
+    int mt, nt;
+    tile_at(p, p.dp_tiles + t, mt, nt);
+    const int tb = mt / p.m_tiles_per_batch;
+    const RowAt at = row_at(p, tb, (int64_t)(mt - tb * p.m_tiles_per_batch) * 256 + row);
+    const int n = nt * BN + col;
+    if (!at.live || n >= p.n) return;
+    float f[8] = {};
+    for (int c = c0; c <= c1; ++c) {
+        const int slot = 2 * c + (first > c * p.cut_each ? 1 : 0);
+        const float4* q = reinterpret_cast<const float4*>(p.part + ((int64_t)slot * 256 + row) * BN + col);
+        const float4 a = q[0], b = q[1];
+        f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
+        f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+    }
+    if (p.bias) {
+        float q[8];
+        load8_any(p.bias, n, p.bias_dtype, p.n - n, p.vec_bias, q);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = __fadd_rn(f[e], q[e]);
+    }
+    finish8<T>(p, f, n, at);
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+struct FewParams {
+    LinParams l;                 // the epilogue's part
+    const uint16_t* x;
+    const uint16_t* w;
+    int64_t xs_b, xs_h, xs_s, w_stride;
+    int k, k_head;
+};
+
+// Few rows (8 NT at most): y^T = w x^T, 16 MT rows of w per CTA.  A lane reads
+// 16-byte runs of w rows (lane / 4) and (lane / 4 + 8), eight channels each, four
+// lanes 64 consecutive bytes, kFewK / 32 runs in flight; x's rows are read with
+// the same assignment of channels to fragment positions (any bijection gives
+// the same sum over k).  Warp i takes every eighth run of kFewK channels, and
+// the eight partial sums meet in shared memory, added in warp order.
+// Bound: HBM, w's bytes.
+constexpr int kFewK = 128;
+
+template <typename T, int MT, int NT>
+__global__ void __launch_bounds__(256) linear_few_kernel(const __grid_constant__ FewParams p) {
+    pdl_wait();
+    pdl_open();
+    constexpr int kU = kFewK / 32;
+    __shared__ float part[8][MT * 16][NT * 8 + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int n0 = blockIdx.x * (16 * MT);
+    const int rows = (int)p.l.rows;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    const uint16_t* wrow[2 * MT];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) wrow[i] = p.w + (int64_t)(n0 + 8 * i + g) * p.w_stride;
+    const uint16_t* xrow[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int r = 8 * j + g, b = r / (int)p.l.tokens;
+        xrow[j] = p.x + b * p.xs_b + (r - b * (int)p.l.tokens) * p.xs_s;
+    }
+    float acc[MT][NT][4] = {};
+    for (int k0 = warp * kFewK; k0 < p.k; k0 += 8 * kFewK) {
+        uint4 wv[kU][2 * MT], xv[kU][NT];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int k = k0 + 32 * u + 8 * t;
+            const bool in = k < p.k;
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i)
+                wv[u][i] = in && n0 + 8 * i + g < p.l.n ? __ldg(reinterpret_cast<const uint4*>(wrow[i] + k)) : zero;
+            const int h = k / p.k_head;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                xv[u][j] = in && 8 * j + g < rows
+                               ? __ldg(reinterpret_cast<const uint4*>(xrow[j] + h * p.xs_h + (k - h * p.k_head)))
+                               : zero;
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const uint32_t a0[4] = {wv[u][2 * i].x, wv[u][2 * i + 1].x, wv[u][2 * i].y, wv[u][2 * i + 1].y};
+                const uint32_t a1[4] = {wv[u][2 * i].z, wv[u][2 * i + 1].z, wv[u][2 * i].w, wv[u][2 * i + 1].w};
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    mma16816<T>(acc[i][j], a0, xv[u][j].x, xv[u][j].y);
+                    mma16816<T>(acc[i][j], a1, xv[u][j].z, xv[u][j].w);
+                }
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) part[warp][16 * i + g + 8 * (e >> 1)][8 * j + 2 * t + (e & 1)] = acc[i][j][e];
+    __syncthreads();
+    // one thread per output element; consecutive threads, consecutive columns of y
+    for (int o = threadIdx.x; o < MT * 16 * NT * 8; o += 256) {
+        const int r = o / (MT * 16), c = o - r * (MT * 16), n = n0 + c;
+        if (r >= rows || n >= p.l.n) continue;
+        float f = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) f += part[q][c][r];
+        const RowAt at = row_at(p.l, 0, r);
+        float v[8];
+        if (p.l.bias) {
+            load8_any(p.l.bias, n, p.l.bias_dtype, 1, false, v);
+            f = __fadd_rn(f, v[0]);
+        }
+        f = act_of(p.l.activation, f);
+        if (p.l.gate) {
+            load8_any(p.l.gate, at.g + n, p.l.gate_dtype, 1, false, v);
+            f = __fmul_rn(f, v[0]);
+        }
+        if (p.l.residual) {
+            load8_any(p.l.residual, at.r + n, F16<T>::kDtype, 1, false, v);
+            f = __fadd_rn(f, v[0]);
+        }
+        const int h = n / p.l.n_head;
+        static_cast<T*>(p.l.y)[at.y + h * p.l.ys_h + (n - h * p.l.n_head)] = F16<T>::one(f);
+    }
+}
+
+template <typename T, int MT, int NT> int launch_few(const FewParams& p, cudaStream_t st) {
+    VCB_CUDA(launch_pdl(linear_few_kernel<T, MT, NT>, dim3((unsigned)((p.l.n + 16 * MT - 1) / (16 * MT))), dim3(256), 0,
+                        st, p));
+    return VCB_OK;
+}
+template <typename T> int launch_few_any(const FewParams& p, cudaStream_t st) {
+    if (p.l.rows <= 8) return launch_few<T, 1, 1>(p, st);
+    if (p.l.rows <= 16) return launch_few<T, 1, 2>(p, st);
+    return launch_few<T, 2, 4>(p, st);
+}
+
+template <typename T, int BN>
+int launch_tiles(const LinParams& p, int grid_pairs, cudaStream_t st) {
+    static bool ready[64] = {};
     using L = Tile<BN>;
     auto kernel = linear_kernel<T, BN>;
     int dev = 0;
@@ -429,27 +641,33 @@ int launch_tiles(LinParams& p, cudaStream_t st) {
     cfg.dynamicSmemBytes = L::kSmem;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (max_pairs[dev] == 0) {
-        VCB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem));
-        cfg.gridDim = dim3(2 * 148);
-        int n = 0;
-        VCB_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
-        if (n < 1) return fail(VCB_ERR_CUDA, "the projection kernel's CTA pairs do not fit on this GPU");
-        max_pairs[dev] = n;
-    }
-    p.n_tiles = (p.n + BN - 1) / BN;
-    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-    cfg.gridDim = dim3((unsigned)(2 * (tiles < max_pairs[dev] ? tiles : max_pairs[dev])));
     cfg.numAttrs = 2;
+    if (!ready[dev]) {
+        VCB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem));
+        ready[dev] = true;
+    }
+    cfg.gridDim = dim3((unsigned)(2 * grid_pairs));
     VCB_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+    if (p.cut_units) {
+        const int tiles = p.cut_units / p.k_chunks;
+        VCB_CUDA(launch_pdl(linear_join_kernel<T, BN>, dim3((unsigned)tiles * (BN / 8)), dim3(256), 0, st, p));
+    }
     return VCB_OK;
 }
 
+// Up to this many rows of x the product streams w through linear_few_kernel.
+constexpr int kFewRows = 32;
+
 struct LinPlan {
     bool pack_x, pack_w;
-    int64_t pitch;               // elements of a packed row
-    size_t off_w, total;
+    int64_t pitch;                        // elements of a packed row
+    int64_t heads, k_head, w_stride;      // operands as the kernels read them
+    int64_t xs_b, xs_h, xs_s;
+    bool few, collapsed;
+    int64_t rows, batches, m_tiles;
+    int bn, chunks_per_head, k_chunks, grid_pairs;
+    int64_t tiles, dp_tiles, cut_units, cut_each;
+    size_t off_w, off_part, total;
 };
 
 LinPlan plan(const vcb_linear_args* a) {
@@ -459,9 +677,62 @@ LinPlan plan(const vcb_linear_args* a) {
     q.pack_w = !on16(a->w) || !tma_stride(a->w_stride, a->n);
     q.pack_x = !on16(a->x) || (a->heads_in > 1 && !by8(a->k_head)) || !tma_stride(a->x_stride_s, a->tokens) ||
                !tma_stride(a->x_stride_h, a->heads_in) || !tma_stride(a->x_stride_b, a->batch);
-    auto r = [](size_t v) { return (v + 255) & ~size_t(255); };
-    q.off_w = q.pack_x ? r((size_t)(a->batch * a->tokens * q.pitch) * 2) : 0;
-    q.total = q.off_w + (q.pack_w ? r((size_t)(a->n * q.pitch) * 2) : 0);
+    q.heads = a->heads_in; q.k_head = a->k_head; q.w_stride = a->w_stride;
+    q.xs_b = a->x_stride_b; q.xs_h = a->x_stride_h; q.xs_s = a->x_stride_s;
+    if (q.pack_x) {                       // a packed row has its heads joined
+        q.heads = 1; q.k_head = k;
+        q.xs_s = q.pitch; q.xs_h = q.pitch; q.xs_b = a->tokens * q.pitch;
+    }
+    if (q.pack_w) q.w_stride = q.pitch;
+    auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
+    q.off_w = q.pack_x ? up((size_t)(a->batch * a->tokens * q.pitch) * 2) : 0;
+    q.off_part = q.total = q.off_w + (q.pack_w ? up((size_t)(a->n * q.pitch) * 2) : 0);
+    // (16-byte runs of a row must not pass its end)
+    q.few = a->batch * a->tokens <= kFewRows && (by8(k) || (q.pack_x && q.pack_w));
+    if (q.few) return q;
+
+    // one walk over batch x tokens where the rows are evenly spaced
+    q.collapsed = q.heads == 1 && (a->batch == 1 || a->tokens == 1 || q.xs_b == a->tokens * q.xs_s);
+    if (q.collapsed && a->tokens == 1 && a->batch > 1) q.xs_s = q.xs_b;
+    q.rows = q.collapsed ? a->batch * a->tokens : a->tokens;
+    q.batches = q.collapsed ? 1 : a->batch;
+    // strides of axes of length one are never taken: any legal value will do
+    const int64_t row = (q.k_head + 7) / 8 * 8;
+    if (q.rows == 1) q.xs_s = row;
+    if (q.heads == 1) q.xs_h = row;
+    if (q.batches == 1) q.xs_b = row;
+    if (a->n == 1) q.w_stride = row * q.heads;
+    q.chunks_per_head = (int)((q.k_head + kBK - 1) / kBK);
+    q.k_chunks = (int)(q.chunks_per_head * q.heads);
+    q.m_tiles = (q.rows + 255) / 256 * q.batches;
+    // Tile width, and whether the tiles of the last, partly filled round are
+    // cut along K.  Cost in clocks: a 64-channel chunk takes 650 / 490 / 410 with
+    // 256 / 128 / 64 columns (the loads of x and w bind the narrow ones); a cut
+    // adds the join, its launch and the partial sums' way through L2.
+    const int64_t pairs = sm_count() / 2;
+    const int clocks[3] = {650, 490, 410}, widths[3] = {256, 128, 64};
+    double best = 0;
+    for (int i = 0; i < 3; ++i) {
+        const int bn = widths[i];
+        const int64_t tiles = q.m_tiles * ((a->n + bn - 1) / bn), rem = tiles % pairs;
+        const double chunk = clocks[i], tile = chunk * q.k_chunks + 1500;
+        const double whole = (double)((tiles + pairs - 1) / pairs) * tile;
+        int64_t each = (rem * q.k_chunks + pairs - 1) / pairs;
+        if (each < 4) each = 4;
+        const double cut = (double)(tiles / pairs) * tile + (double)each * chunk + 1500 + 5000 + (double)rem * bn * 0.4;
+        const bool use_cut = rem && each < q.k_chunks && cut < whole;
+        const double cost = use_cut ? cut : whole;
+        if (i && cost >= best) continue;
+        best = cost;
+        q.bn = bn;
+        q.tiles = tiles;
+        q.dp_tiles = use_cut ? tiles - rem : tiles;
+        q.cut_units = use_cut ? rem * q.k_chunks : 0;
+        q.cut_each = use_cut ? each : 1;
+        const int64_t shares = use_cut ? (q.cut_units + each - 1) / each : 0;
+        q.grid_pairs = (int)(q.dp_tiles >= pairs ? pairs : use_cut ? shares : tiles);
+    }
+    if (q.cut_units) q.total = q.off_part + (size_t)2 * pairs * 256 * q.bn * 4;
     return q;
 }
 
@@ -474,21 +745,20 @@ int linear_run(const vcb_linear_args* a, cudaStream_t st) {
     const int64_t k = a->heads_in * a->k_head;
     const void* x = a->x;
     const void* w = a->w;
-    int64_t heads = a->heads_in, k_head = a->k_head, w_stride = a->w_stride;
-    int64_t xb = a->x_stride_b, xh = a->x_stride_h, xs = a->x_stride_s;
+    char* ws = static_cast<char*>(a->workspace);
+    if (q.tiles >= (1ll << 30) || (q.tiles / 74 + 2) * q.k_chunks >= (1ll << 31))
+        return fail(VCB_ERR_INVALID_ARGUMENT, "product too large for the projection kernel's tile counters");
     if (q.pack_x || q.pack_w) {
         PackParams pk{};
         pk.channels = (int)k;
         pk.pitch = (int)q.pitch;
-        char* ws = static_cast<char*>(a->workspace);
         int64_t blocks = 0;
         if (q.pack_x) {
             const int64_t rows = a->batch * a->tokens;
-            pk.side[0] = {static_cast<const uint16_t*>(x), reinterpret_cast<uint16_t*>(ws), rows, a->tokens, xb, xs, 1,
-                          0, xh, (int)a->k_head};
+            pk.side[0] = {static_cast<const uint16_t*>(x), reinterpret_cast<uint16_t*>(ws), rows, a->tokens,
+                          a->x_stride_b, a->x_stride_s, 1, 0, a->x_stride_h, (int)a->k_head};
             blocks += (rows + 7) / 8;
             x = ws;
-            xs = q.pitch; xh = k; xb = a->tokens * q.pitch;
         }
         pk.end[0] = blocks;
         if (q.pack_w) {
@@ -496,54 +766,13 @@ int linear_run(const vcb_linear_args* a, cudaStream_t st) {
                           a->w_stride, 1, 0, k, (int)k};
             blocks += (a->n + 7) / 8;
             w = ws + q.off_w;
-            w_stride = q.pitch;
         }
         pk.end[1] = pk.end[2] = blocks;
-        if (q.pack_x) { heads = 1; k_head = k; }      // a packed row has its heads joined
         VCB_CUDA(launch_pack(pk, st));
     }
     LinParams p;
     memset(&p, 0, sizeof(p));
     const bool bf16 = a->dtype == VCB_BF16;
-    // one walk over batch x tokens where the rows are evenly spaced
-    p.collapsed = heads == 1 && (a->batch == 1 || a->tokens == 1 || xb == a->tokens * xs);
-    if (p.collapsed && a->tokens == 1 && a->batch > 1) xs = xb;
-    const int64_t rows = p.collapsed ? a->batch * a->tokens : a->tokens;
-    const int64_t batches = p.collapsed ? 1 : a->batch;
-    // strides of axes of length one are never taken: any legal value will do
-    const int64_t row = (k_head + 7) / 8 * 8;
-    if (rows == 1) xs = row;
-    if (heads == 1) xh = row;
-    if (batches == 1) xb = row;
-    if (a->n == 1) w_stride = row * heads;
-    {
-        const cuuint64_t dims[4] = {(cuuint64_t)k_head, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batches};
-        const cuuint64_t strides[3] = {(cuuint64_t)xs * 2, (cuuint64_t)xh * 2, (cuuint64_t)xb * 2};
-        const cuuint32_t box[4] = {kBK, 128, 1, 1};
-        int rc = make_map16(&p.tm_x, x, bf16, 4, dims, strides, box);
-        if (rc) return rc;
-    }
-    const int64_t m_per_batch = (rows + 255) / 256;
-    const int64_t m_tiles = m_per_batch * batches;
-    // Tile width: 256 columns need the fewest loads per product; narrower ones
-    // give small products a tile for more of the SM pairs.
-    const int pairs = sm_count() / 2;
-    int bn = 256;
-    if (m_tiles * ((a->n + 255) / 256) < pairs) bn = m_tiles * ((a->n + 127) / 128) < pairs ? 64 : 128;
-    {
-        const cuuint64_t dims[3] = {(cuuint64_t)k_head, (cuuint64_t)heads, (cuuint64_t)a->n};
-        const cuuint64_t strides[2] = {(cuuint64_t)row * 2, (cuuint64_t)w_stride * 2};
-        const cuuint32_t box[3] = {kBK, 1, (cuuint32_t)(bn / 2)};
-        int rc = make_map16(&p.tm_w, w, bf16, 3, dims, strides, box);
-        if (rc) return rc;
-    }
-    p.chunks_per_head = (int)((k_head + kBK - 1) / kBK);
-    p.k_chunks = (int)(p.chunks_per_head * heads);
-    if (m_tiles * ((a->n + 63) / 64) >= (1ll << 30) || ((m_tiles * ((a->n + bn - 1) / bn) + 73) / 74) * p.k_chunks >= (1ll << 31))
-        return fail(VCB_ERR_INVALID_ARGUMENT, "product too large for the projection kernel's tile counters");
-    p.m_tiles = (int)m_tiles;
-    p.m_tiles_per_batch = (int)m_per_batch;
-    p.rows = rows;
     p.tokens = a->tokens;
     p.n = (int)a->n;
     p.n_head = (int)a->n_head;
@@ -557,14 +786,52 @@ int linear_run(const vcb_linear_args* a, cudaStream_t st) {
     p.vec_bias = on16(a->bias);
     p.vec_gate = on16(a->gate) && by8(a->gate_stride_b) && by8(a->gate_stride_s);
     p.status = a->status;
-    if (bf16) {
-        if (bn == 256) return launch_tiles<__nv_bfloat16, 256>(p, st);
-        if (bn == 128) return launch_tiles<__nv_bfloat16, 128>(p, st);
-        return launch_tiles<__nv_bfloat16, 64>(p, st);
+    if (q.few) {
+        FewParams f;
+        f.l = p;
+        f.l.rows = a->batch * a->tokens;
+        f.l.collapsed = 1;
+        f.x = static_cast<const uint16_t*>(x);
+        f.w = static_cast<const uint16_t*>(w);
+        f.xs_b = q.xs_b; f.xs_h = q.xs_h; f.xs_s = q.xs_s; f.w_stride = q.w_stride;
+        f.k = (int)(by8(k) ? k : q.pitch);
+        f.k_head = (int)(q.heads > 1 ? q.k_head : f.k);
+        return bf16 ? launch_few_any<__nv_bfloat16>(f, st) : launch_few_any<__half>(f, st);
     }
-    if (bn == 256) return launch_tiles<__half, 256>(p, st);
-    if (bn == 128) return launch_tiles<__half, 128>(p, st);
-    return launch_tiles<__half, 64>(p, st);
+    {
+        const cuuint64_t dims[4] = {(cuuint64_t)q.k_head, (cuuint64_t)q.rows, (cuuint64_t)q.heads, (cuuint64_t)q.batches};
+        const cuuint64_t strides[3] = {(cuuint64_t)q.xs_s * 2, (cuuint64_t)q.xs_h * 2, (cuuint64_t)q.xs_b * 2};
+        const cuuint32_t box[4] = {kBK, 128, 1, 1};
+        int rc = make_map16(&p.tm_x, x, bf16, 4, dims, strides, box);
+        if (rc) return rc;
+    }
+    {
+        const cuuint64_t dims[3] = {(cuuint64_t)q.k_head, (cuuint64_t)q.heads, (cuuint64_t)a->n};
+        const cuuint64_t head_stride = (cuuint64_t)((q.k_head + 7) / 8 * 8) * 2;
+        const cuuint64_t strides[2] = {head_stride, (cuuint64_t)q.w_stride * 2};
+        const cuuint32_t box[3] = {kBK, 1, (cuuint32_t)(q.bn / 2)};
+        int rc = make_map16(&p.tm_w, w, bf16, 3, dims, strides, box);
+        if (rc) return rc;
+    }
+    p.chunks_per_head = q.chunks_per_head;
+    p.k_chunks = q.k_chunks;
+    p.m_tiles = (int)q.m_tiles;
+    p.n_tiles = (int)((a->n + q.bn - 1) / q.bn);
+    p.m_tiles_per_batch = (int)((q.rows + 255) / 256);
+    p.rows = q.rows;
+    p.collapsed = q.collapsed;
+    p.dp_tiles = (int)q.dp_tiles;
+    p.cut_units = (int)q.cut_units;
+    p.cut_each = (int)q.cut_each;
+    p.part = reinterpret_cast<float*>(ws + q.off_part);
+    if (bf16) {
+        if (q.bn == 256) return launch_tiles<__nv_bfloat16, 256>(p, q.grid_pairs, st);
+        if (q.bn == 128) return launch_tiles<__nv_bfloat16, 128>(p, q.grid_pairs, st);
+        return launch_tiles<__nv_bfloat16, 64>(p, q.grid_pairs, st);
+    }
+    if (q.bn == 256) return launch_tiles<__half, 256>(p, q.grid_pairs, st);
+    if (q.bn == 128) return launch_tiles<__half, 128>(p, q.grid_pairs, st);
+    return launch_tiles<__half, 64>(p, q.grid_pairs, st);
 }
 
 }  // namespace vcb
