@@ -147,17 +147,17 @@ template <int HD, int NQ> struct WinTile {
     static constexpr int kStages = NQ == 2 ? (HD == 128 ? 5 : 8) : (HD == 128 ? 2 : 5);
     static constexpr uint32_t kOffKV = NQ * kBytes;
     static constexpr uint32_t kOffBars = kOffKV + kStages * kBytes;
-    static constexpr int kNumBars = 1 + 2 * kStages + 3 * 2 + 1 + 1;
+    static constexpr int kNumBars = 1 + 2 * kStages + 4 * 2 + 1 + 1;
     static constexpr uint32_t kOffMisc = kOffBars + kNumBars * 8;
     static constexpr uint32_t kSmem = kOffMisc + 16;
-    static constexpr int kThreads = 128 + 128 * NQ;
+    static constexpr int kThreads = 128 + 256 * NQ;
     static constexpr int kCtas = NQ == 2 ? 1 : 2;                // per SM
     // tensor memory: S (P over it) and O of each query tile
     static constexpr uint32_t kCols = NQ == 2 ? 512 : 256;
     static constexpr uint32_t kColO = NQ * 128;
     // setmaxnreg shares: control warps, softmax warps
-    static constexpr int kRegsCtl = NQ == 2 ? 80 : 64, kRegsSoft = NQ == 2 ? 208 : 192;
-    static constexpr int kRegSplit = 128 * kRegsCtl + 128 * NQ * kRegsSoft;
+    static constexpr int kRegsCtl = 64, kRegsSoft = NQ == 2 ? 104 : 88;
+    static constexpr int kRegSplit = 128 * kRegsCtl + 256 * NQ * kRegsSoft;
     static_assert(kSmem <= 232448 / kCtas - (kCtas - 1) * 1024, "shared memory of one CTA");
 };
 
@@ -166,7 +166,8 @@ struct WinBars {
     uint64_t* kv_full;    // [stages]
     uint64_t* kv_empty;   // [stages]  the stage's products are done
     uint64_t* s_full;     // [2]  S_w(j) is there, and PV_w(j-1) done
-    uint64_t* p_full;     // [2]  P_w(j) is there, O_w rescaled
+    uint64_t* p_half;     // [2]  P_w(j) of the keys 0-31 and 64-95 is there, O_w rescaled
+    uint64_t* p_full;     // [2]  all of P_w(j)
     uint64_t* o_full;     // [2]  the last PV_w is done
     uint64_t* v_last;     // [1]  the V tile that holds the last key landed; warp 2 clears the rows behind it
                           //      and arrives on that stage's kv_full itself
@@ -179,6 +180,7 @@ template <typename L> __device__ __forceinline__ WinBars win_bars(uint8_t* smem)
     r.kv_full = b; b += L::kStages;
     r.kv_empty = b; b += L::kStages;
     r.s_full = b; b += 2;
+    r.p_half = b; b += 2;
     r.p_full = b; b += 2;
     r.o_full = b; b += 2;
     r.v_last = b; b += 1;
@@ -228,37 +230,76 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
         ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
-// D[128 x N] (+)= A B, A and B in shared memory
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+// D[128 x N] (+)= A B, A and B in shared memory.  The whole warp runs the issue
+// loop and one elected lane issues: its operands then stay in uniform registers.
+// (A lone thread's operands were moved there one by one before every MMA, and
+// next to the busy softmax warps of its scheduler an MMA of 64 clocks took 80
+// to 100 to issue.)  Descriptors differ in the low word only.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                       uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "mov.b64 da, {%1, %3};\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}"
+        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 // the same with A in tensor memory
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                       uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// 32 lanes x 32 columns from r[OFF .. OFF + 31]
-template <int OFF, int N> __device__ __forceinline__ void tmem_st32_at(uint32_t taddr, const uint32_t (&r)[N]) {
-    static_assert(OFF + 32 <= N, "range");
+// 16 lanes x (N columns, and N columns SPLIT behind): thread t < 16 of the warp
+// has lane base + t and the first run, thread t + 16 the same lane and the second
+template <int SPLIT> __device__ __forceinline__ void tmem_ld16x2_32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+        "tcgen05.ld.sync.aligned.16x32bx2.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32], %33;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr), "n"(SPLIT));
+}
+template <int SPLIT> __device__ __forceinline__ void tmem_st16x2_32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x32bx2.x32.b32 [%0], %33, {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
         "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+          "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
+          "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "n"(SPLIT)
+        : "memory");
+}
+template <int SPLIT, int OFF, int N> __device__ __forceinline__ void tmem_st16x2_16(uint32_t taddr, const uint32_t (&r)[N]) {
+    static_assert(OFF + 16 <= N, "range");
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x32bx2.x16.b32 [%0], %17, {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+        "%13, %14, %15, %16};"
         ::"r"(taddr), "r"(r[OFF + 0]), "r"(r[OFF + 1]), "r"(r[OFF + 2]), "r"(r[OFF + 3]), "r"(r[OFF + 4]),
           "r"(r[OFF + 5]), "r"(r[OFF + 6]), "r"(r[OFF + 7]), "r"(r[OFF + 8]), "r"(r[OFF + 9]), "r"(r[OFF + 10]),
-          "r"(r[OFF + 11]), "r"(r[OFF + 12]), "r"(r[OFF + 13]), "r"(r[OFF + 14]), "r"(r[OFF + 15]),
-          "r"(r[OFF + 16]), "r"(r[OFF + 17]), "r"(r[OFF + 18]), "r"(r[OFF + 19]), "r"(r[OFF + 20]),
-          "r"(r[OFF + 21]), "r"(r[OFF + 22]), "r"(r[OFF + 23]), "r"(r[OFF + 24]), "r"(r[OFF + 25]),
-          "r"(r[OFF + 26]), "r"(r[OFF + 27]), "r"(r[OFF + 28]), "r"(r[OFF + 29]), "r"(r[OFF + 30]),
-          "r"(r[OFF + 31])
+          "r"(r[OFF + 11]), "r"(r[OFF + 12]), "r"(r[OFF + 13]), "r"(r[OFF + 14]), "r"(r[OFF + 15]), "n"(SPLIT)
+        : "memory");
+}
+
+// commit of the elected lane's MMAs (the same lane every time)
+__device__ __forceinline__ void mma_commit_elected(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(smem_u32(bar))
         : "memory");
 }
 
@@ -293,28 +334,35 @@ __device__ void win_producer(const WinParams& p, const WinItem& it, int fix, uin
 }
 
 template <typename T, int HD, int NQ>
-__device__ void win_mma(const WinItem& it, uint8_t* smem, const WinBars& B, uint32_t tmem, volatile int* abort) {
+__device__ void win_mma(const WinItem& it, uint8_t* smem, const WinBars& B, uint32_t tmem0, volatile int* abort) {
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem0, 0);      // uniform
     using L = WinTile<HD, NQ>;
     constexpr uint32_t idesc_qk = idesc_f16<T>(128, kKT), idesc_pv = idesc_f16<T>(128, HD, true);
-    const uint64_t q0 = smem_desc_k128(smem), k0 = smem_desc_k128(smem + L::kOffKV);
+    const uint64_t k64 = smem_desc_k128(smem + L::kOffKV);
+    const uint32_t hi = (uint32_t)(k64 >> 32), q0 = (uint32_t)smem_desc_k128(smem), k0 = (uint32_t)k64;
     // V tile as the N-major operand: 64-channel blocks a box apart (leading
-    // offset), groups of 8 keys 1024 bytes apart (stride offset)
-    const uint64_t v0 = (k0 & ~(0x3FFFull << 16)) | ((uint64_t)(L::kBox >> 4) << 16);
+    // offset, bits [16, 30)), groups of 8 keys 1024 bytes apart (stride offset)
+    const uint32_t v0 = (k0 & 0xffffu) | ((L::kBox >> 4) << 16);
     auto qk = [&](int w, int s) {
+        const uint32_t q = q0 + w * (L::kBytes >> 4), k = k0 + s * (L::kBytes >> 4);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
             const uint32_t step = (kk / 4) * (L::kBox >> 4) + 2 * (kk % 4);
-            mma_ss(tmem + 128 * w, q0 + w * (L::kBytes >> 4) + step, k0 + s * (L::kBytes >> 4) + step, idesc_qk, kk > 0);
+            mma_ss(tmem + 128 * w, q + step, k + step, hi, idesc_qk, kk > 0);
         }
+    };
+    auto pv = [&](int w, int s, int kk, bool accumulate) {
+        mma_ts(tmem + L::kColO + 128 * w, tmem + 128 * w + 8 * kk, v0 + s * (L::kBytes >> 4) + 128 * kk, hi, idesc_pv,
+               accumulate);
     };
     bool ok = mbar_wait(B.q_full, 0, abort) && mbar_wait(&B.kv_full[0], 0, abort);
     if (ok) {
         tc_fence_after();
         for (int w = 0; w < it.nq; ++w) {
             qk(w, 0);
-            mma_commit(&B.s_full[w]);
+            mma_commit_elected(&B.s_full[w]);
         }
-        mma_commit(&B.kv_empty[0]);
+        mma_commit_elected(&B.kv_empty[0]);
     }
     for (int j = 0; ok && j < it.count; ++j) {
         const int gv = 2 * j + 1, gk = 2 * j + 2;
@@ -322,133 +370,151 @@ __device__ void win_mma(const WinItem& it, uint8_t* smem, const WinBars& B, uint
         const bool more = j + 1 < it.count;
         ok = mbar_wait(&B.kv_full[sv], (gv / L::kStages) & 1, abort);
         for (int w = 0; ok && w < it.nq; ++w) {
+            if (!mbar_wait(&B.p_half[w], j & 1, abort)) { ok = false; break; }
+            tc_fence_after();
+            pv(w, sv, 0, j > 0); pv(w, sv, 1, true); pv(w, sv, 4, true); pv(w, sv, 5, true);
             if (!mbar_wait(&B.p_full[w], j & 1, abort)) { ok = false; break; }
             tc_fence_after();
-#pragma unroll
-            for (int kk = 0; kk < kKT / 16; ++kk)
-                mma_ts(tmem + L::kColO + 128 * w, tmem + 128 * w + 8 * kk, v0 + sv * (L::kBytes >> 4) + 128 * kk, idesc_pv,
-                       j > 0 || kk > 0);
-            if (w == it.nq - 1) mma_commit(&B.kv_empty[sv]);
+            pv(w, sv, 2, true); pv(w, sv, 3, true); pv(w, sv, 6, true); pv(w, sv, 7, true);
+            if (w == it.nq - 1) mma_commit_elected(&B.kv_empty[sv]);
             if (more) {
                 if (w == 0 && !mbar_wait(&B.kv_full[sk], (gk / L::kStages) & 1, abort)) { ok = false; break; }
                 tc_fence_after();
                 qk(w, sk);
-                mma_commit(&B.s_full[w]);
-                if (w == it.nq - 1) mma_commit(&B.kv_empty[sk]);
+                mma_commit_elected(&B.s_full[w]);
+                if (w == it.nq - 1) mma_commit_elected(&B.kv_empty[sk]);
             } else {
-                mma_commit(&B.o_full[w]);
+                mma_commit_elected(&B.o_full[w]);
             }
         }
     }
-    mma_commit(B.drain);
+    mma_commit_elected(B.drain);
     drain_wait(B.drain, 0);
 }
 
 // Bits [a, b) of the 32-key word that starts at key 32 w of a tile.
 __device__ __forceinline__ uint32_t bits_below(int x) { return x <= 0 ? 0u : x >= 32 ? 0xffffffffu : (1u << x) - 1u; }
 
+// Warp (quarter, sub) of query tile w owns rows 32 quarter + 16 sub + [0, 16);
+// lanes t and t + 16 share a row, keys [0, 64) and [64, 128) of each tile.
 template <typename T, int HD, int NQ>
 __device__ void win_softmax(const WinParams& p, const WinItem& it, uint8_t* smem, const WinBars& B, uint32_t tmem, int w,
-                            int quarter, int lane, volatile int* abort) {
+                            int quarter, int sub, int lane, volatile int* abort) {
     using L = WinTile<HD, NQ>;
+    const int half = lane >> 4;
     const int64_t tile_row = it.row0 + 128 * w;
-    const int64_t row = tile_row + quarter * 32 + lane;
+    const int64_t row0 = tile_row + quarter * 32 + sub * 16, row = row0 + (lane & 15);
     const bool valid = row < p.sq;
-    const bool warp_live = tile_row + quarter * 32 < p.sq;
+    const bool warp_live = row0 < p.sq;
     const int64_t last = min(tile_row + 128, p.sq) - 1;
     const Seen none{0, 0, 0};
     const Seen mine = valid ? seen_at(p, row + it.offset, it.len) : none;
-    const Seen first = seen_at(p, tile_row + it.offset, it.len), end = seen_at(p, last + it.offset, it.len);
-    const uint32_t trow = tmem + ((uint32_t)(quarter * 32) << 16);
+    const bool sees = mine.sink > 0 || mine.hi > mine.lo;
+    // tiles that all rows of the query tile see whole: keys up to sink_all, and
+    // from lo_all up to hi_all
+    int sink_all, lo_all, hi_all;
+    {
+        const Seen first = seen_at(p, tile_row + it.offset, it.len), end = seen_at(p, last + it.offset, it.len);
+        sink_all = first.sink;
+        hi_all = first.hi;
+        lo_all = end.lo <= first.sink ? 0 : end.lo;
+    }
+    const uint32_t trow = tmem + ((uint32_t)(quarter * 32 + sub * 16) << 16);
     const uint32_t ts = trow + 128 * w, to = trow + L::kColO + 128 * w;
+    const float c = p.c;
     float m = -INFINITY, den = 0.0f;
     for (int j = 0; j < it.count; ++j) {
         if (!mbar_wait(&B.s_full[w], j & 1, abort)) return;
         tc_fence_after();
-        if (warp_live) {
-            uint32_t r[128];
-            tmem_ld32_at<0>(ts, r);
-            tmem_ld32_at<32>(ts + 32, r);
-            tmem_ld32_at<64>(ts + 64, r);
-            tmem_ld32_at<96>(ts + 96, r);
-            tmem_wait_ld();
-            const int k0 = it.tile(j) * kKT, k1 = k0 + kKT;
-            // all rows of the query tile see all keys of this one
-            const bool full = k1 <= first.sink || (k1 <= first.hi && (k0 >= end.lo || end.lo <= first.sink));
-            if (!full) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int o = k0 + 32 * q;
-                    const uint32_t seen = bits_below(mine.sink - o) | (bits_below(mine.hi - o) & ~bits_below(mine.lo - o));
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (!(seen & (1u << e))) r[32 * q + e] = 0xff800000u;
-                }
-            }
-            float mx[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mx[e] = fmaxf(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
-#pragma unroll
-            for (int t = 1; t < 8; ++t)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    mx[e] = fmax3(mx[e], __uint_as_float(r[16 * t + 2 * e]), __uint_as_float(r[16 * t + 2 * e + 1]));
-            const float top =
-                __fmul_rn(fmaxf(fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]), mx[6]), mx[7]), p.c);
-            const float m_new = top > m + 8.0f ? top : m;
-            const float alpha = m_new == m ? 1.0f : ex2_ftz(m - m_new);
-            const bool moved = __any_sync(0xffffffffu, m_new != m);
-            const float ref = m_new == -INFINITY ? 0.0f : m_new;
-            const float2 cc = make_float2(p.c, p.c), rr = make_float2(-ref, -ref);
-            uint32_t pk[64];
-#pragma unroll
-            for (int e = 0; e < 64; ++e) {
-                const float2 x = ffma2(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), cc, rr);
-                pk[e] = F16<T>::two(ex2_ftz(x.x), ex2_ftz(x.y));
-            }
-            tmem_st32_at<0>(ts, pk);
-            tmem_st32_at<32>(ts + 32, pk);
-            if (moved && j > 0) {                                // PV_w(j-1) is done: s_full follows it
-#pragma unroll 1
-                for (int q = 0; q < HD / 32; ++q) {
-                    uint32_t o[32];
-                    tmem_ld32_at<0>(to + 32 * q, o);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__fmul_rn(__uint_as_float(o[e]), alpha));
-                    tmem_st32_at<0>(to + 32 * q, o);
-                }
-            }
-            tmem_wait_st();
+        if (!warp_live) {
             tc_fence_before();
             __syncwarp();
+            mbar_arrive_if(&B.p_half[w], lane == 0);
             mbar_arrive_if(&B.p_full[w], lane == 0);
-            float2 sum[4] = {};
-#pragma unroll
-            for (int e = 0; e < 64; ++e) sum[e & 3] = fadd2(sum[e & 3], F16<T>::both(pk[e]));
-            const float2 s2 = fadd2(fadd2(sum[0], sum[1]), fadd2(sum[2], sum[3]));
-            den = __fmaf_rn(den, alpha, __fadd_rn(s2.x, s2.y));
-            m = m_new;
-        } else {
-            tc_fence_before();
-            __syncwarp();
-            mbar_arrive_if(&B.p_full[w], lane == 0);
+            continue;
         }
+        uint32_t r[64];
+        tmem_ld16x2_at<0>(ts, r);                                // keys 0-31 | 64-95
+        tmem_ld16x2_at<32>(ts + 32, r);                          // keys 32-63 | 96-127
+        tmem_wait_ld();
+        const int k0 = it.tile(j) * kKT, k1 = k0 + kKT;
+        if (!(k1 <= sink_all || (k1 <= hi_all && k0 >= lo_all))) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int o = k0 + 64 * half + 32 * q;
+                const uint32_t seen = bits_below(mine.sink - o) | (bits_below(mine.hi - o) & ~bits_below(mine.lo - o));
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (!(seen & (1u << e))) r[32 * q + e] = 0xff800000u;
+            }
+        }
+        float mx[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+#pragma unroll
+        for (int t = 1; t < 8; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                mx[e] = fmax3(mx[e], __uint_as_float(r[8 * t + 2 * e]), __uint_as_float(r[8 * t + 2 * e + 1]));
+        float top = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
+        top = __fmul_rn(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)), c);
+        const float m_new = top > m + 8.0f ? top : m;
+        const float alpha = m_new == m ? 1.0f : ex2_ftz(m - m_new);
+        const bool moved = __any_sync(0xffffffffu, m_new != m);
+        const float ref = m_new == -INFINITY ? 0.0f : m_new;
+        const float2 cc = make_float2(c, c), rr = make_float2(-ref, -ref);
+        if (moved && j > 0) {                                    // PV_w(j-1) is done: s_full follows it
+#pragma unroll 1
+            for (int q = 0; q < HD / 64; ++q) {
+                uint32_t o[32];
+                tmem_ld16x2_32<HD / 2>(to + 32 * q, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__fmul_rn(__uint_as_float(o[e]), alpha));
+                tmem_st16x2_32<HD / 2>(to + 32 * q, o);
+            }
+        }
+        uint32_t pk[32];
+        auto weights = [&](int e) {
+            const float2 x = ffma2(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), cc, rr);
+            pk[e] = F16<T>::two(ex2_ftz(x.x), ex2_ftz(x.y));
+        };
+#pragma unroll
+        for (int e = 0; e < 16; ++e) weights(e);
+        tmem_st16x2_16<32, 0>(ts, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        mbar_arrive_if(&B.p_half[w], lane == 0);
+#pragma unroll
+        for (int e = 16; e < 32; ++e) weights(e);
+        tmem_st16x2_16<32, 16>(ts + 16, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        mbar_arrive_if(&B.p_full[w], lane == 0);
+        float2 sum[2] = {};
+#pragma unroll
+        for (int e = 0; e < 32; ++e) sum[e & 1] = fadd2(sum[e & 1], F16<T>::both(pk[e]));
+        sum[0] = fadd2(sum[0], sum[1]);
+        den = __fmaf_rn(den, alpha, __fadd_rn(sum[0].x, sum[0].y));
+        m = m_new;
     }
     if (!warp_live) return;
+    den += __shfl_xor_sync(0xffffffffu, den, 16);
     if (it.count > 0) {
         if (!mbar_wait(&B.o_full[w], 0, abort)) return;
         tc_fence_after();
     }
-    const bool sees = mine.sink > 0 || mine.hi > mine.lo;
+    const int ch0 = half * (HD / 2);                             // this lane's channels: ch0 + 32 q + [0, 32)
     if (p.splits > 1) {
         const int64_t at = ((int64_t)it.split * (gridDim.x / p.splits / p.q_tiles) + it.bh) * p.sq + row;
         if (it.count > 0) {
-            float4* dst = reinterpret_cast<float4*>(p.part + at * HD);
+            float4* dst = reinterpret_cast<float4*>(p.part + at * HD + ch0);
 #pragma unroll 1
-            for (int q = 0; q < HD / 32; ++q) {
+            for (int q = 0; q < HD / 64; ++q) {
                 uint32_t o[32];
-                tmem_ld32_at<0>(to + 32 * q, o);
+                tmem_ld16x2_32<HD / 2>(to + 32 * q, o);
                 tmem_wait_ld();
                 if (valid) {
 #pragma unroll
@@ -458,7 +524,7 @@ __device__ void win_softmax(const WinParams& p, const WinItem& it, uint8_t* smem
                 }
             }
         }
-        if (valid) p.part_ml[at] = make_float2(m, den);
+        if (valid && half == 0) p.part_ml[at] = make_float2(m, den);
         return;
     }
     // out = O / den; a row that sees nothing is 0
@@ -466,39 +532,42 @@ __device__ void win_softmax(const WinParams& p, const WinItem& it, uint8_t* smem
     T* out = static_cast<T*>(p.out) + it.b * p.os[0] + it.h * p.os[1] + row * p.os[2];
     bool bad = false;
 #pragma unroll 1
-    for (int q = 0; q < HD / 32; ++q) {
+    for (int q = 0; q < HD / 64; ++q) {
         uint32_t o[32];
         if (it.count > 0) {
-            tmem_ld32_at<0>(to + 32 * q, o);
+            tmem_ld16x2_32<HD / 2>(to + 32 * q, o);
             tmem_wait_ld();
         }
-        float f[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-            f[e] = sees ? __fmul_rn(__uint_as_float(o[e]), inv) : 0.0f;
-            bad |= !finite_f(f[e]);
+            const float f = sees ? __fmul_rn(__uint_as_float(o[e]), inv) : 0.0f;
+            bad |= !finite_f(f);
+            o[e] = __float_as_uint(f);
         }
+        const int ch = ch0 + 32 * q;
         if (valid) {
             if (p.vec_out) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (32 * q + 8 * e < p.d)
-                        *reinterpret_cast<uint4*>(out + 32 * q + 8 * e) =
-                            make_uint4(F16<T>::two(f[8 * e], f[8 * e + 1]), F16<T>::two(f[8 * e + 2], f[8 * e + 3]),
-                                       F16<T>::two(f[8 * e + 4], f[8 * e + 5]), F16<T>::two(f[8 * e + 6], f[8 * e + 7]));
+                    if (ch + 8 * e < p.d) {
+                        auto two = [&](int i) {
+                            return F16<T>::two(__uint_as_float(o[8 * e + i]), __uint_as_float(o[8 * e + i + 1]));
+                        };
+                        *reinterpret_cast<uint4*>(out + ch + 8 * e) = make_uint4(two(0), two(2), two(4), two(6));
+                    }
             } else {
 #pragma unroll
                 for (int e = 0; e < 32; ++e)
-                    if (32 * q + e < p.d) out[32 * q + e] = F16<T>::one(f[e]);
+                    if (ch + e < p.d) out[ch + e] = F16<T>::one(__uint_as_float(o[e]));
             }
         }
     }
     // rows with a NaN or infinity among the tiles' keys (or no finite logit)
     unsigned again = __ballot_sync(0xffffffffu, valid && sees && bad);
+    again = (again | (again >> 16)) & 0xffffu;
     if (again) {
-        float* qrow = reinterpret_cast<float*>(smem + w * L::kBytes) + 128 * quarter;    // Q_w is no longer read
-        for (; again; again &= again - 1)
-            window_row<T>(p, it.b, it.h, tile_row + quarter * 32 + __ffs(again) - 1, qrow, lane);
+        float* qrow = reinterpret_cast<float*>(smem + w * L::kBytes) + 128 * (2 * quarter + sub);   // Q_w is no longer read
+        for (; again; again &= again - 1) window_row<T>(p, it.b, it.h, row0 + __ffs(again) - 1, qrow, lane);
     }
 }
 
@@ -515,7 +584,7 @@ __global__ void __launch_bounds__(WinTile<HD, NQ>::kThreads, WinTile<HD, NQ>::kC
     const WinBars B = win_bars<L>(smem);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
     volatile int* abort = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;      // warp: uniform
     const WinItem it = win_item<NQ>(p);
     if (threadIdx.x == 0) {
         mbar_init(B.q_full, 1);
@@ -525,7 +594,8 @@ __global__ void __launch_bounds__(WinTile<HD, NQ>::kThreads, WinTile<HD, NQ>::kC
         }
         for (int w = 0; w < 2; ++w) {
             mbar_init(&B.s_full[w], 1);
-            mbar_init(&B.p_full[w], 4);
+            mbar_init(&B.p_half[w], 8);
+            mbar_init(&B.p_full[w], 8);
             mbar_init(&B.o_full[w], 1);
         }
         mbar_init(B.v_last, 1);
@@ -552,7 +622,7 @@ __global__ void __launch_bounds__(WinTile<HD, NQ>::kThreads, WinTile<HD, NQ>::kC
         reg_dealloc<L::kRegsCtl>();
         if (it.count > 0) {
             if (warp == 0 && lane == 0) win_producer<L>(p, it, fix, smem, B, abort);
-            if (warp == 1 && lane == 0) win_mma<T, HD, NQ>(it, smem, B, tmem, abort);
+            if (warp == 1) win_mma<T, HD, NQ>(it, smem, B, tmem, abort);
             if (warp == 2 && fix >= 0) {
                 const int s = (2 * fix + 1) % L::kStages;
                 if (mbar_wait(B.v_last, 0, abort)) {
@@ -570,8 +640,8 @@ __global__ void __launch_bounds__(WinTile<HD, NQ>::kThreads, WinTile<HD, NQ>::kC
         }
     } else {
         reg_alloc<L::kRegsSoft>();
-        const int w = (warp - 4) >> 2;
-        if (w < it.nq) win_softmax<T, HD, NQ>(p, it, smem, B, tmem, w, warp & 3, lane, abort);
+        const int w = (warp - 4) >> 3;
+        if (w < it.nq) win_softmax<T, HD, NQ>(p, it, smem, B, tmem, w, warp & 3, ((warp - 4) >> 2) & 1, lane, abort);
     }
     tc_fence_before();
     __syncwarp();
