@@ -11,8 +11,8 @@
 // queries the bytes of K and V.
 //
 // Work decomposition.  A CTA owns NQ (1 or 2) tiles of 128 queries of one
-// head, and with few queries one of `splits` parts of their key tiles; parts
-// are joined by window_join_kernel in a fixed order.  Per key tile and query
+// head; items that would not fill the last round of CTAs are cut along their
+// keys, and window_join_kernel joins the parts in a fixed order.  Per key tile and query
 // tile: S = Q K^T into tensor memory (tcgen05, 128 x 128), the softmax
 // warpgroup of the query tile (one thread per row) turns S into P = 2^(s - m)
 // in 16 bits over S's own columns, and O += P V adds onto the row's sums in
@@ -54,9 +54,11 @@ struct WinParams {
     int causal, has_offset, d;
     float scale;
     float c;                                 // scale log2(e)
-    int q_tiles, splits, vec_out;
-    float* part;                             // [splits][batch heads][sq][HD] sums, splits > 1
-    float2* part_ml;                         // [splits][batch heads][sq] maximum (log2) and row sum
+    int q_tiles, vec_out;
+    int whole, splits;                       // items of one CTA; parts of each item behind them
+    int64_t part_rows;                       // rows of those items
+    float* part;                             // [splits][part_rows][HD] sums
+    float2* part_ml;                         // [splits][part_rows] maximum (log2) and row sum
     int32_t* status;
 };
 
@@ -192,8 +194,9 @@ template <typename L> __device__ __forceinline__ WinBars win_bars(uint8_t* smem)
 // key tiles begin .. begin + count - 1 of its list, tiles 0 .. n1 - 1 and then
 // from w0 on.
 struct WinItem {
-    int64_t b, h, bh, row0, len, offset;
-    int split, nq, n1, w0, begin, count;
+    int64_t b, h, row0, len, offset;
+    int64_t part_at;             // first row among the parts' rows, -1 for a whole item
+    int nq, n1, w0, begin, count;
     __device__ __forceinline__ int tile(int j) const {
         const int i = begin + j;
         return i < n1 ? i : w0 + i - n1;
@@ -201,12 +204,19 @@ struct WinItem {
 };
 template <int NQ> __device__ __forceinline__ WinItem win_item(const WinParams& p) {
     WinItem it;
-    uint32_t r = blockIdx.x;
-    it.split = r % p.splits; r /= p.splits;
-    const int qt = p.q_tiles - 1 - (int)(r % p.q_tiles);        // late (longer) causal tiles first
-    it.bh = r / p.q_tiles;
-    it.b = it.bh / p.heads;
-    it.h = it.bh - it.b * p.heads;
+    int r = blockIdx.x, split = 0, splits = 1;
+    it.part_at = -1;
+    if (r >= p.whole && p.splits > 1) {
+        const int o = r - p.whole;
+        splits = p.splits;
+        split = o % splits;
+        it.part_at = split * p.part_rows + (int64_t)(o / splits) * (128 * NQ);
+        r = p.whole + o / splits;
+    }
+    const int qt = p.q_tiles - 1 - r % p.q_tiles;               // late (longer) causal tiles first
+    const int64_t bh = r / p.q_tiles;
+    it.b = bh / p.heads;
+    it.h = bh - it.b * p.heads;
     it.row0 = (int64_t)qt * (128 * NQ);
     it.nq = NQ == 2 && it.row0 + 128 < p.sq ? 2 : 1;
     it.len = keys_of(p, it.b);
@@ -218,8 +228,8 @@ template <int NQ> __device__ __forceinline__ WinItem win_item(const WinParams& p
     it.w0 = max(it.n1, a.lo / kKT);
     const int w1 = z.hi > a.lo ? (z.hi + kKT - 1) / kKT : 0;
     const int total = it.n1 + max(0, w1 - it.w0);
-    it.begin = (int)((int64_t)total * it.split / p.splits);
-    it.count = (int)((int64_t)total * (it.split + 1) / p.splits) - it.begin;
+    it.begin = (int)((int64_t)total * split / splits);
+    it.count = (int)((int64_t)total * (split + 1) / splits) - it.begin;
     return it;
 }
 
@@ -507,8 +517,8 @@ __device__ void win_softmax(const WinParams& p, const WinItem& it, uint8_t* smem
         tc_fence_after();
     }
     const int ch0 = half * (HD / 2);                             // this lane's channels: ch0 + 32 q + [0, 32)
-    if (p.splits > 1) {
-        const int64_t at = ((int64_t)it.split * (gridDim.x / p.splits / p.q_tiles) + it.bh) * p.sq + row;
+    if (it.part_at >= 0) {
+        const int64_t at = it.part_at + (row - it.row0);
         if (it.count > 0) {
             float4* dst = reinterpret_cast<float4*>(p.part + at * HD + ch0);
 #pragma unroll 1
@@ -655,15 +665,18 @@ __global__ void __launch_bounds__(WinTile<HD, NQ>::kThreads, WinTile<HD, NQ>::kC
 
 // One warp per row: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) den_s over
 // the parts in order.
-template <typename T, int HD>
-__global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ WinParams p, int64_t rows) {
+template <typename T, int HD, int NQ>
+__global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ WinParams p) {
     pdl_wait();
     pdl_open();
     __shared__ float qrow[8][128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t r = (int64_t)blockIdx.x * 8 + warp;
-    if (r >= rows) return;
-    const int64_t bh = r / p.sq, i = r - bh * p.sq, b = bh / p.heads, h = bh - b * p.heads;
+    const int item = p.whole + (int)(r / (128 * NQ));
+    const int64_t bh = item / p.q_tiles, b = bh / p.heads, h = bh - b * p.heads;
+    const int64_t i = (int64_t)(p.q_tiles - 1 - item % p.q_tiles) * (128 * NQ) + r % (128 * NQ);
+    if (i >= p.sq) return;
+    const int64_t rows = p.part_rows;
     const int64_t len = keys_of(p, b);
     const Seen s = seen_at(p, i + (p.has_offset ? p.q_offset : len - p.sq), len);
     const bool sees = s.sink > 0 || s.hi > s.lo;
@@ -692,6 +705,7 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
 
 struct WinPlan {
     int hd, nq, q_tiles, splits;
+    int64_t items, whole;
     int pitch;                   // channels of a packed row
     bool pack[3];                // Q, K, V
     size_t off[3], off_part, off_ml, total;
@@ -716,16 +730,21 @@ WinPlan plan(const vcb_window_args* a) {
         const int64_t sink = tiles(a->sinks);
         if (sink + span < all) t = sink + span;
     }
-    // Parts: as many as make the last wave of CTAs full, counting what a CTA
-    // spends outside its tiles (about four tiles' time) and the join.
-    const int64_t slots = (int64_t)sm_count() * (r.nq == 1 ? 2 : 1), items = bh * r.q_tiles;
+    // Items that do not fill the last round of CTAs are cut along their keys,
+    // into as many parts as make the time of the rounds least: a part costs its
+    // tiles and about four tiles' time, the join of all parts about four more.
+    const int64_t slots = (int64_t)sm_count() * (r.nq == 1 ? 2 : 1);
+    r.items = bh * r.q_tiles;
+    const int64_t rest = r.items % slots;
     r.splits = 1;
-    int64_t best = 0;
-    for (int64_t s = 1; s <= 32 && s <= t && items * (s - 1) < 2 * slots; ++s) {
-        const int64_t cost = (items * s + slots - 1) / slots * ((t + s - 1) / s + 4) + (s > 1 ? 4 : 0);
-        if (s == 1 || cost < best) {
+    r.whole = r.items;
+    int64_t best = rest ? t + 4 : 0;
+    for (int64_t s = 2; rest && s <= 32 && s <= t; ++s) {
+        const int64_t cost = (rest * s + slots - 1) / slots * ((t + s - 1) / s + 4) + 4;
+        if (cost < best) {
             best = cost;
             r.splits = (int)s;
+            r.whole = r.items - rest;
         }
     }
     const void* base[3] = {a->q, a->k, a->v};
@@ -740,14 +759,15 @@ WinPlan plan(const vcb_window_args* a) {
         if (r.pack[i]) o += up((size_t)(bh * n * r.pitch) * 2);
     }
     r.off_part = o;
-    if (r.splits > 1) o += up((size_t)(r.splits * bh * a->sq * r.hd) * 4);
+    const int64_t part_rows = r.splits * (r.items - r.whole) * rows;
+    o += up((size_t)(part_rows * r.hd) * 4);
     r.off_ml = o;
-    if (r.splits > 1) o += up((size_t)(r.splits * bh * a->sq) * 8);
+    o += up((size_t)part_rows * 8);
     r.total = o;
     return r;
 }
 
-template <typename T, int HD, int NQ> int launch(const WinParams& p, int64_t items, cudaStream_t st) {
+template <typename T, int HD, int NQ> int launch(const WinParams& p, const WinPlan& r, cudaStream_t st) {
     using L = WinTile<HD, NQ>;
     static bool ready[64] = {};
     auto kernel = window_kernel<T, HD, NQ>;
@@ -764,16 +784,15 @@ template <typename T, int HD, int NQ> int launch(const WinParams& p, int64_t ite
                         fa.numRegs, L::kThreads, L::kRegSplit);
         ready[dev] = true;
     }
-    VCB_CUDA(launch_pdl(window_kernel<T, HD, NQ>, dim3((unsigned)items), dim3(L::kThreads), L::kSmem, st, p));
-    if (p.splits > 1) {
-        const int64_t rows = items / p.splits / p.q_tiles * p.sq;
-        VCB_CUDA(launch_pdl(window_join_kernel<T, HD>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p, rows));
-    }
+    const int64_t cut = r.items - r.whole;
+    VCB_CUDA(launch_pdl(window_kernel<T, HD, NQ>, dim3((unsigned)(r.whole + cut * r.splits)), dim3(L::kThreads), L::kSmem,
+                        st, p));
+    if (cut) VCB_CUDA(launch_pdl(window_join_kernel<T, HD, NQ>, dim3((unsigned)(cut * 16 * NQ)), dim3(256), 0, st, p));
     return VCB_OK;
 }
-template <typename T> int launch_any(const WinParams& p, const WinPlan& r, int64_t items, cudaStream_t st) {
-    if (r.hd == 128) return r.nq == 1 ? launch<T, 128, 1>(p, items, st) : launch<T, 128, 2>(p, items, st);
-    return r.nq == 1 ? launch<T, 64, 1>(p, items, st) : launch<T, 64, 2>(p, items, st);
+template <typename T> int launch_any(const WinParams& p, const WinPlan& r, cudaStream_t st) {
+    if (r.hd == 128) return r.nq == 1 ? launch<T, 128, 1>(p, r, st) : launch<T, 128, 2>(p, r, st);
+    return r.nq == 1 ? launch<T, 64, 1>(p, r, st) : launch<T, 64, 2>(p, r, st);
 }
 
 }  // namespace
@@ -782,8 +801,8 @@ size_t window_workspace_bytes(const vcb_window_args* a) { return plan(a).total; 
 
 int window_run(const vcb_window_args* a, cudaStream_t st) {
     const WinPlan r = plan(a);
-    const int64_t bh = a->batch * a->heads, items = bh * r.q_tiles * r.splits;
-    if (items >= (1ll << 31)) return fail(VCB_ERR_INVALID_ARGUMENT, "too many query tiles for one grid");
+    const int64_t bh = a->batch * a->heads;
+    if (r.items >= (1ll << 30)) return fail(VCB_ERR_INVALID_ARGUMENT, "too many query tiles for one grid");
     WinParams p;
     memset(&p, 0, sizeof(p));
     p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out;
@@ -796,7 +815,9 @@ int window_run(const vcb_window_args* a, cudaStream_t st) {
     p.causal = a->causal; p.has_offset = a->has_offset; p.q_offset = a->q_offset;
     p.d = a->d; p.scale = a->scale;
     p.c = (float)((double)a->scale * 1.4426950408889634);
-    p.q_tiles = r.q_tiles; p.splits = r.splits;
+    p.q_tiles = r.q_tiles;
+    p.whole = (int)r.whole; p.splits = r.splits;
+    p.part_rows = (r.items - r.whole) * 128 * r.nq;
     p.vec_out = on16(a->out) && by8(a->d) && by8(a->out_stride[0]) && by8(a->out_stride[1]) && by8(a->out_stride[2]);
     char* ws = static_cast<char*>(a->workspace);
     p.part = reinterpret_cast<float*>(ws + r.off_part);
@@ -833,7 +854,7 @@ int window_run(const vcb_window_args* a, cudaStream_t st) {
     }
     if (blocks >= (1ll << 31)) return fail(VCB_ERR_INVALID_ARGUMENT, "too many rows for one grid");
     if (blocks) VCB_CUDA(launch_pack(pk, st));
-    return a->dtype == VCB_BF16 ? launch_any<__nv_bfloat16>(p, r, items, st) : launch_any<__half>(p, r, items, st);
+    return a->dtype == VCB_BF16 ? launch_any<__nv_bfloat16>(p, r, st) : launch_any<__half>(p, r, st);
 }
 
 }  // namespace vcb
