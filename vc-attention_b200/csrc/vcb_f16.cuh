@@ -90,13 +90,18 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const __grid_constant__ 
     const int64_t o = row / s.tokens, t = row - o * s.tokens;
     const int64_t b = o / s.inner, i = o - b * s.inner;
     const uint16_t* src = s.src + b * s.s_b + i * s.s_i + t * s.s_s;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(s.dst + row * p.pitch);
-    auto get = [&](int c) -> uint32_t {
-        if (c >= p.channels) return 0u;
-        const int h = c / s.head_dim;
-        return src[h * s.s_h + (c - h * s.head_dim)];
-    };
-    for (int c = 2 * (threadIdx.x & 31); c < p.pitch; c += 64) dst[c / 2] = get(c) | (get(c + 1) << 16);
+    uint4* dst = reinterpret_cast<uint4*>(s.dst + row * p.pitch);
+    // eight channels per lane, all reads in flight before the 16-byte store
+    for (int c = 8 * (threadIdx.x & 31); c < p.pitch; c += 256) {
+        uint32_t v[8];
+        int h = c / s.head_dim, k = c - h * s.head_dim;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[e] = c + e < p.channels ? src[h * s.s_h + k] : 0u;
+            if (++k == s.head_dim) { k = 0; ++h; }
+        }
+        dst[c / 8] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+    }
 }
 cudaError_t launch_pack(const PackParams& p, cudaStream_t st) {
     return launch_pdl(pack_rows_kernel, dim3((unsigned)p.end[2]), dim3(256), 0, st, p);

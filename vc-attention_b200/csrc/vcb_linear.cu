@@ -85,7 +85,7 @@ struct LinParams {
     void* y;
     int bias_dtype, gate_dtype;
     int64_t gs_b, gs_s, rs_b, rs_s, ys_b, ys_h, ys_s;
-    int vec_y, vec_r, vec_bias, vec_gate;
+    int vec;                     // y, bias, gate and residual in whole, aligned 16-byte runs
     int32_t* status;
 };
 
@@ -232,11 +232,30 @@ __device__ void lin_mma(const LinParams& p, uint8_t* smem, const LinBars& B, con
     drain_wait(B.drain, 0);
 }
 
+// 0.5 y (1 + erf(y / sqrt 2)) without the cancellation for y < 0: with
+// z = |y| / sqrt 2 and t = 1 / (1 + 0.45 z), erfc(z) = t q(t) exp(-z^2), q a degree-7
+// fit to erfc(z) exp(z^2) / t over z in [0, 60] (least squares reweighted towards
+// the largest relative error, which is 6e-7).  No branches: erfcf's two made this
+// the longest part of a small product (51 us of 771 x 2049 x 1147).
+__device__ __forceinline__ float gelu_erf(float y) {
+    const float z = 0.70710678118654752f * fabsf(y);
+    const float t = __fdividef(1.0f, __fmaf_rn(0.45f, z, 1.0f));
+    float q = 0.0671004429f;
+    q = __fmaf_rn(q, t, -0.242869869f);
+    q = __fmaf_rn(q, t, 0.216092497f);
+    q = __fmaf_rn(q, t, 0.0311580617f);
+    q = __fmaf_rn(q, t, 0.194682702f);
+    q = __fmaf_rn(q, t, 0.225934967f);
+    q = __fmaf_rn(q, t, 0.254018039f);
+    q = __fmaf_rn(q, t, 0.253882557f);
+    const float e = 0.5f * t * q * __expf(-z * z);
+    return y * (y < 0.0f ? e : 1.0f - e);
+}
+
 __device__ __forceinline__ float act_of(int kind, float y) {
     switch (kind) {
         case VCB_ACT_SILU: return __fdividef(y, 1.0f + __expf(-y));
-        // 0.5 y (1 + erf(y / sqrt 2)), without the cancellation for y < 0
-        case VCB_ACT_GELU: return 0.5f * y * erfcf(-0.70710678118654752f * y);
+        case VCB_ACT_GELU: return gelu_erf(y);
         // 0.5 y (1 + tanh u) = y / (1 + exp(-2 u)), u = sqrt(2/pi) (y + 0.044715 y^3)
         case VCB_ACT_GELU_TANH: {
             const float u2 = 1.5957691216057308f * y * __fmaf_rn(0.044715f * y, y, 1.0f);
@@ -247,35 +266,19 @@ __device__ __forceinline__ float act_of(int kind, float y) {
     }
 }
 
-// Eight consecutive values of a bias, gate or residual row as floats; columns
-// at or behind `limit` are not read.
-__device__ __forceinline__ void load8_any(const void* p, int64_t i, int dtype, int valid, bool vec, float* o) {
-    if (vec && valid >= 8) {
-        if (dtype == VCB_F32) {
-            const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-            const float4 a = f[0], b = f[1];
-            o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w; o[4] = b.x; o[5] = b.y; o[6] = b.z; o[7] = b.w;
-        } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float2 f;
-                if (dtype == VCB_F16) f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-                else f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]));
-                o[2 * e] = f.x; o[2 * e + 1] = f.y;
-            }
-        }
+// Eight consecutive values of a bias or gate row as floats (16-byte aligned).
+__device__ __forceinline__ void load8_any(const void* p, int64_t i, int dtype, float* o) {
+    if (dtype == VCB_F32) {
+        const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+        const float4 a = f[0], b = f[1];
+        o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w; o[4] = b.x; o[5] = b.y; o[6] = b.z; o[7] = b.w;
     } else {
+        const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float f = 0.0f;
-            if (e < valid) {
-                if (dtype == VCB_F32) f = static_cast<const float*>(p)[i + e];
-                else if (dtype == VCB_F16) f = __half2float(static_cast<const __half*>(p)[i + e]);
-                else f = __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i + e]);
-            }
-            o[e] = f;
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = dtype == VCB_F16 ? F16<__half>::both(w[e]) : F16<__nv_bfloat16>::both(w[e]);
+            o[2 * e] = f.x; o[2 * e + 1] = f.y;
         }
     }
 }
@@ -294,41 +297,66 @@ __device__ __forceinline__ RowAt row_at(const LinParams& p, int64_t b, int64_t r
     return {b * p.ys_b + s * p.ys_s, b * p.gs_b + s * p.gs_s, b * p.rs_b + s * p.rs_s, row < p.rows};
 }
 
-// Eight accumulated columns n .. n + 7 of one row: act, gate, residual, store.
-// f holds the sums with the bias added.
+// Four rows of a 32 x 32 block, eight columns n .. n + 7 of each (16-byte runs):
+// all reads of the gate and the residual come before the first store, since
+// the output may be the residual itself and would hold them back.
 template <typename T>
-__device__ __forceinline__ void finish8(const LinParams& p, float* f, int n, const RowAt& at) {
-    const int valid = p.n - n;
-    if (p.activation != VCB_ACT_NONE) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = act_of(p.activation, f[e]);
-    }
-    if (p.gate) {
-        float q[8];
-        load8_any(p.gate, at.g + n, p.gate_dtype, valid, p.vec_gate, q);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(f[e], q[e]);
-    }
+__device__ __forceinline__ void finish_rows(const LinParams& p, float (&f)[4][8], const float* bias, int n,
+                                            const RowAt (&at)[4], int h, int64_t col) {
+    uint4 res[4];
     if (p.residual) {
-        float q[8];
-        load8_any(p.residual, at.r + n, F16<T>::kDtype, valid, p.vec_r, q);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = __fadd_rn(f[e], q[e]);
+        for (int i = 0; i < 4; ++i)
+            if (at[i].live) res[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.residual) + at[i].r + n);
     }
-    T* y = static_cast<T*>(p.y) + at.y;
-    if (p.vec_y && valid >= 8) {
-        const int h = n / p.n_head;
-        *reinterpret_cast<uint4*>(y + h * p.ys_h + (n - h * p.n_head)) =
-            make_uint4(F16<T>::two(f[0], f[1]), F16<T>::two(f[2], f[3]), F16<T>::two(f[4], f[5]),
-                       F16<T>::two(f[6], f[7]));
-    } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < valid) {
-                const int h = (n + e) / p.n_head;
-                y[h * p.ys_h + (n + e - h * p.n_head)] = F16<T>::one(f[e]);
+    for (int i = 0; i < 4; ++i) {
+        float gate[8];
+        if (p.gate && at[i].live) load8_any(p.gate, at[i].g + n, p.gate_dtype, gate);
+        if (p.bias) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[i][e] = __fadd_rn(f[i][e], bias[e]);
+        }
+        if (p.activation != VCB_ACT_NONE) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[i][e] = act_of(p.activation, f[i][e]);
+        }
+        if (p.gate) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[i][e] = __fmul_rn(f[i][e], gate[e]);
+        }
+        if (p.residual) {
+            const uint32_t w[4] = {res[i].x, res[i].y, res[i].z, res[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 q = F16<T>::both(w[e]);
+                f[i][2 * e] = __fadd_rn(f[i][2 * e], q.x);
+                f[i][2 * e + 1] = __fadd_rn(f[i][2 * e + 1], q.y);
             }
+        }
     }
+    T* y = static_cast<T*>(p.y) + h * p.ys_h + col;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (at[i].live)
+            *reinterpret_cast<uint4*>(y + at[i].y) =
+                make_uint4(F16<T>::two(f[i][0], f[i][1]), F16<T>::two(f[i][2], f[i][3]), F16<T>::two(f[i][4], f[i][5]),
+                           F16<T>::two(f[i][6], f[i][7]));
+}
+
+__device__ __forceinline__ float load1_any(const void* p, int64_t i, int dtype) {
+    if (dtype == VCB_F32) return static_cast<const float*>(p)[i];
+    if (dtype == VCB_F16) return __half2float(static_cast<const __half*>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+// One sum's epilogue, for outputs off the 16-byte grid and the small kernels:
+// column n = head h, channel col.
+template <typename T>
+__device__ __forceinline__ float finish1(const LinParams& p, float f, float bias, int n, const RowAt& at, float residual) {
+    f = act_of(p.activation, __fadd_rn(f, bias));
+    if (p.gate) f = __fmul_rn(f, load1_any(p.gate, at.g + n, p.gate_dtype));
+    return p.residual ? __fadd_rn(f, residual) : f;
 }
 
 template <typename T, int BN>
@@ -372,28 +400,58 @@ __device__ void lin_epilogue(const LinParams& p, uint8_t* smem, const LinBars& B
                     make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
                                 __uint_as_float(r[4 * j + 3]));
             __syncwarp();
-            const int n = nt * BN + side * kHalfCols + ch * 32 + q8;
-            if (n < p.n) {
-                float bias[8];
-                if (p.bias && !part) load8_any(p.bias, n, p.bias_dtype, p.n - n, p.vec_bias, bias);
+            const int n0 = nt * BN + side * kHalfCols + ch * 32;
+            if (part) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int row = r0 + 8 * i;
-                    const float4 a = stage[row * 8 + ((q8 >> 2) ^ (row & 7))];
-                    const float4 d = stage[row * 8 + (((q8 >> 2) + 1) ^ (row & 7))];
                     if (!at[i].live) continue;
-                    if (part) {
-                        float4* to = reinterpret_cast<float4*>(part + (int64_t)(8 * i) * BN + ch * 32);
-                        to[0] = a;
-                        to[1] = d;
-                        continue;
-                    }
-                    float f[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
-                    if (p.bias) {
+                    float4* to = reinterpret_cast<float4*>(part + (int64_t)(8 * i) * BN + ch * 32);
+                    to[0] = stage[row * 8 + ((q8 >> 2) ^ (row & 7))];
+                    to[1] = stage[row * 8 + (((q8 >> 2) + 1) ^ (row & 7))];
+                }
+            } else if (p.vec) {
+                const int n = n0 + q8;
+                if (n < p.n) {
+                    float bias[8], f[4][8];
+                    if (p.bias) load8_any(p.bias, n, p.bias_dtype, bias);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = __fadd_rn(f[e], bias[e]);
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = r0 + 8 * i;
+                        const float4 a = stage[row * 8 + ((q8 >> 2) ^ (row & 7))];
+                        const float4 d = stage[row * 8 + (((q8 >> 2) + 1) ^ (row & 7))];
+                        f[i][0] = a.x; f[i][1] = a.y; f[i][2] = a.z; f[i][3] = a.w;
+                        f[i][4] = d.x; f[i][5] = d.y; f[i][6] = d.z; f[i][7] = d.w;
                     }
-                    finish8<T>(p, f, n, at[i]);
+                    const int h = n / p.n_head;
+                    finish_rows<T>(p, f, bias, n, at, h, n - h * p.n_head);
+                }
+            } else {
+                // one column per lane: 64-byte runs whatever the alignment, eight
+                // rows' reads in flight
+                const int n = n0 + lane;
+                const bool in = n < p.n;
+                const float bias = p.bias && in ? load1_any(p.bias, n, p.bias_dtype) : 0.0f;
+                const int h = n / p.n_head, col = n - h * p.n_head;
+                const float* one = reinterpret_cast<const float*>(stage);
+#pragma unroll 1
+                for (int r8 = 0; r8 < 32; r8 += 8) {
+                    RowAt q[8];
+                    float res[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        q[i] = row_at(p, tb, row0 - r0 + r8 + i);
+                        res[i] = p.residual && in && q[i].live
+                                     ? F16<T>::to(static_cast<const T*>(p.residual)[q[i].r + n]) : 0.0f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int row = r8 + i;
+                        const float f = one[row * 32 + (((lane >> 2) ^ (row & 7)) << 2) + (lane & 3)];
+                        if (in && q[i].live)
+                            static_cast<T*>(p.y)[q[i].y + h * p.ys_h + col] =
+                                F16<T>::one(finish1<T>(p, f, bias, n, q[i], res[i]));
+                    }
                 }
             }
             __syncwarp();
@@ -484,13 +542,26 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
         f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
         f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
     }
-    if (p.bias) {
-        float q[8];
-        load8_any(p.bias, n, p.bias_dtype, p.n - n, p.vec_bias, q);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = __fadd_rn(f[e], q[e]);
+    for (int e = 0; e < 8; ++e) {
+        if (n + e >= p.n) break;
+        const float bias = p.bias ? load1_any(p.bias, n + e, p.bias_dtype) : 0.0f;
+        const float res = p.residual ? F16<T>::to(static_cast<const T*>(p.residual)[at.r + n + e]) : 0.0f;
+        f[e] = finish1<T>(p, f[e], bias, n + e, at, res);
     }
-    finish8<T>(p, f, n, at);
+    T* y = static_cast<T*>(p.y) + at.y;
+    if (p.vec) {
+        const int h = n / p.n_head;
+        *reinterpret_cast<uint4*>(y + h * p.ys_h + (n - h * p.n_head)) =
+            make_uint4(F16<T>::two(f[0], f[1]), F16<T>::two(f[2], f[3]), F16<T>::two(f[4], f[5]), F16<T>::two(f[6], f[7]));
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (n + e >= p.n) break;
+        const int h = (n + e) / p.n_head;
+        y[h * p.ys_h + (n + e - h * p.n_head)] = F16<T>::one(f[e]);
+    }
 }
 
 template <typename T>
@@ -591,22 +662,11 @@ __global__ void __launch_bounds__(256) linear_few_kernel(const __grid_constant__
 #pragma unroll
         for (int q = 0; q < 8; ++q) f += part[q][c][r];
         const RowAt at = row_at(p.l, 0, r);
-        float v[8];
-        if (p.l.bias) {
-            load8_any(p.l.bias, n, p.l.bias_dtype, 1, false, v);
-            f = __fadd_rn(f, v[0]);
-        }
-        f = act_of(p.l.activation, f);
-        if (p.l.gate) {
-            load8_any(p.l.gate, at.g + n, p.l.gate_dtype, 1, false, v);
-            f = __fmul_rn(f, v[0]);
-        }
-        if (p.l.residual) {
-            load8_any(p.l.residual, at.r + n, F16<T>::kDtype, 1, false, v);
-            f = __fadd_rn(f, v[0]);
-        }
+        const float bias = p.l.bias ? load1_any(p.l.bias, n, p.l.bias_dtype) : 0.0f;
+        const float res = p.l.residual ? F16<T>::to(static_cast<const T*>(p.l.residual)[at.r + n]) : 0.0f;
         const int h = n / p.l.n_head;
-        static_cast<T*>(p.l.y)[at.y + h * p.l.ys_h + (n - h * p.l.n_head)] = F16<T>::one(f);
+        static_cast<T*>(p.l.y)[at.y + h * p.l.ys_h + (n - h * p.l.n_head)] =
+            F16<T>::one(finish1<T>(p.l, f, bias, n, at, res));
     }
 }
 
@@ -781,10 +841,10 @@ int linear_run(const vcb_linear_args* a, cudaStream_t st) {
     p.gate = a->gate; p.gate_dtype = a->gate_dtype; p.gs_b = a->gate_stride_b; p.gs_s = a->gate_stride_s;
     p.residual = a->residual; p.rs_b = a->residual_stride_b; p.rs_s = a->residual_stride_s;
     p.y = a->y; p.ys_b = a->y_stride_b; p.ys_h = a->y_stride_h; p.ys_s = a->y_stride_s;
-    p.vec_y = on16(a->y) && by8(a->n_head) && by8(a->y_stride_b) && by8(a->y_stride_h) && by8(a->y_stride_s);
-    p.vec_r = on16(a->residual) && by8(a->residual_stride_b) && by8(a->residual_stride_s);
-    p.vec_bias = on16(a->bias);
-    p.vec_gate = on16(a->gate) && by8(a->gate_stride_b) && by8(a->gate_stride_s);
+    p.vec = on16(a->y) && by8(a->n_head) && by8(a->y_stride_b) && by8(a->y_stride_h) && by8(a->y_stride_s) &&
+            (!a->bias || on16(a->bias)) &&
+            (!a->gate || (on16(a->gate) && by8(a->gate_stride_b) && by8(a->gate_stride_s))) &&
+            (!a->residual || (on16(a->residual) && by8(a->residual_stride_b) && by8(a->residual_stride_s)));
     p.status = a->status;
     if (q.few) {
         FewParams f;

@@ -30,7 +30,7 @@ struct RopeSide {                    // Q or K
     const void* x;
     void* y;
     const void* w;                   // [d] or null
-    int w_dtype;
+    int w_dtype, w_vec;              // w_vec: 16-byte aligned
     int heads;
     int chunks;                      // warps that share a token's heads
     int64_t xs_b, xs_h, xs_s, ys_b, ys_h, ys_s;
@@ -86,9 +86,12 @@ template <> struct Vec<__half> {
 template <> struct Vec<__nv_bfloat16> {
     static constexpr int N = 8;
     static __device__ __forceinline__ void unpack(const uint4& u, float* f) {
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+        const uint32_t h[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { const float2 v = __bfloat1622float2(h[i]); f[2 * i] = v.x; f[2 * i + 1] = v.y; }
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(h[i] << 16);
+            f[2 * i + 1] = __uint_as_float(h[i] & 0xffff0000u);
+        }
     }
     static __device__ __forceinline__ uint4 pack(const float* f) {
         uint4 u;
@@ -99,11 +102,11 @@ template <> struct Vec<__nv_bfloat16> {
     }
 };
 
-// n consecutive table entries starting at p + i
+// N consecutive fp32 entries p[i ..]; entries at or behind `limit` read as 0
 template <int N>
 __device__ __forceinline__ void load_table(const float* p, int i, int limit, bool vec, float* o) {
     if (vec && i + N <= limit) {
-        if (N % 4 == 0) {
+        if constexpr (N % 4 == 0) {
 #pragma unroll
             for (int e = 0; e < N; e += 4) {
                 const float4 f = __ldg(reinterpret_cast<const float4*>(p + i + e));
@@ -122,15 +125,48 @@ __device__ __forceinline__ void load_table(const float* p, int i, int limit, boo
     }
 }
 
+// N consecutive weights from w[i]; ones without weights
+template <int N>
+__device__ __forceinline__ void load_weights(const RopeSide& s, int i, float* o) {
+    if (!s.w) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] = 1.0f;
+    } else if (s.w_dtype == VCB_F32 && s.w_vec) {
+        load_table<N>(static_cast<const float*>(s.w), i, i + N, true, o);
+    } else if (s.w_vec) {
+        uint32_t u[N / 2];
+        const uint16_t* w = static_cast<const uint16_t*>(s.w) + i;
+        if constexpr (N == 8) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(w));
+            u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w;
+        } else {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(w));
+            u[0] = v.x; u[1] = v.y;
+        }
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) {
+            const float2 f = s.w_dtype == VCB_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&u[e]))
+                                                  : make_float2(__uint_as_float(u[e] << 16),
+                                                                __uint_as_float(u[e] & 0xffff0000u));
+            o[2 * e] = f.x; o[2 * e + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] = load_as_float(s.w, i + e, s.w_dtype);
+    }
+}
+
 // 16-byte vectors, LPR lanes per row.  Needs d, the strides and the base
 // pointers in whole vectors and, for half-split pairs, rotary / 2 too.
+// Weight and angle are multiplied once per token: with A = w cos, B = -+ w' sin
+// (w' the partner's weight) a channel is r (x A + x' B), r the row's 1 / rms.
 template <typename T, int LPR, bool INTERLEAVED>
-__global__ void __launch_bounds__(32 * kWarps) rope_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(32 * kWarps, 4) rope_kernel(const __grid_constant__ RopeParams p) {
     pdl_wait();
     pdl_open();
-    constexpr int N = Vec<T>::N;
+    constexpr int N = Vec<T>::N, P = N / 2;
     constexpr int kRows = 32 / LPR;                  // rows per vector load of the warp
-    constexpr int A = INTERLEAVED ? N / 2 : N;       // angles per lane
+    constexpr int A = INTERLEAVED ? P : N;           // angles per lane
     const int lane = threadIdx.x & 31, li = lane % LPR, sub = lane / LPR;
     const int chunks = p.side[0].chunks + p.side[1].chunks;
     const int block = blockIdx.x / chunks;
@@ -153,59 +189,91 @@ __global__ void __launch_bounds__(32 * kWarps) rope_kernel(const __grid_constant
         const int h = h0 + u * kRows;
         raw[u] = has && h < sd.heads ? load16(x + h * sd.xs_h) : make_uint4(0, 0, 0, 0);
     }
-    // the token's angles, once for all rows: a0 is this lane's first
-    const bool turned = s < p.rows;
-    const int half = turned ? p.half : 0;
-    int a0 = INTERLEAVED ? c / 2 : (c >= half ? c - half : c);
-    const bool rot = INTERLEAVED ? a0 < half : c < 2 * half;
-    float cs[A], sn[A];
-    if (rot && has) {
-        const int64_t t = b * p.ts_b + s * p.ts_s;
-        load_table<A>(p.cos + t, a0, half, p.table_vec, cs);
-        load_table<A>(p.sin + t, a0, half, p.table_vec, sn);
-    }
+    // the token's angles and the weights, once for all rows
+    const int half = s < p.rows ? p.half : 0;
+    const bool low = INTERLEAVED || c < half;        // half-split: this lane's channels are the first of their pairs
+    const int a0 = INTERLEAVED ? c / 2 : (low ? c : c - half);
+    const bool rot = has && (INTERLEAVED ? a0 < half : c < 2 * half);
+    const bool all = rot && a0 + A <= half;          // every channel of this lane turns
+    const int shift = half / (INTERLEAVED ? 1 : N);  // half-split: lanes between partners
+    const int peer = INTERLEAVED || !rot ? li : (low ? li + shift : li - shift);
     float w[N];
+    float2 ca[P], cb[P];                             // A and B of channel pairs 2e, 2e + 1
+    {
+        float cs[A], sn[A], wp[N];
+        if (has) load_weights<N>(sd, c, w);
+        if (rot) {
+            const int64_t t = b * p.ts_b + s * p.ts_s;
+            load_table<A>(p.cos + t, a0, half, p.table_vec, cs);
+            load_table<A>(p.sin + t, a0, half, p.table_vec, sn);
+            if (!INTERLEAVED) load_weights<N>(sd, peer * N, wp);
 #pragma unroll
-    for (int e = 0; e < N; ++e) w[e] = sd.w && has ? load_as_float(sd.w, c + e, sd.w_dtype) : 1.0f;
+            for (int e = 0; e < P; ++e) {
+                if (INTERLEAVED) {
+                    ca[e] = make_float2(__fmul_rn(w[2 * e], cs[e]), __fmul_rn(w[2 * e + 1], cs[e]));
+                    cb[e] = make_float2(-__fmul_rn(w[2 * e + 1], sn[e]), __fmul_rn(w[2 * e], sn[e]));
+                } else {
+                    const float sg = low ? -1.0f : 1.0f;
+                    ca[e] = make_float2(__fmul_rn(w[2 * e], cs[2 * e % A]), __fmul_rn(w[2 * e + 1], cs[(2 * e + 1) % A]));
+                    cb[e] = make_float2(__fmul_rn(sg * wp[2 * e], sn[2 * e % A]),
+                                        __fmul_rn(sg * wp[2 * e + 1], sn[(2 * e + 1) % A]));
+                }
+            }
+        }
+    }
     const float inv_d = 1.0f / (float)p.d;
+    const bool warp_all = __all_sync(0xffffffffu, all);      // the common case: no choice per channel
+    T* to = y + h0 * sd.ys_h;
+    const int64_t step = kRows * sd.ys_h;
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) {
+    for (int u = 0; u < kLoads; ++u, to += step) {
         float f[N];
         Vec<T>::unpack(raw[u], f);
+        float r = 1.0f;
         if (p.norm) {
-            float ss = 0.0f;
+            float2 s2 = make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int e = 0; e < N; ++e) ss = __fmaf_rn(f[e], f[e], ss);
+            for (int e = 0; e < P; ++e) {
+                const float2 v = make_float2(f[2 * e], f[2 * e + 1]);
+                s2 = ffma2(v, v, s2);
+            }
+            float ss = __fadd_rn(s2.x, s2.y);
 #pragma unroll
             for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float r = __frsqrt_rn(__fmaf_rn(ss, inv_d, p.eps));
+            r = rsqrtf(__fmaf_rn(ss, inv_d, p.eps));
+        }
+        const float2 rr = make_float2(r, r);
+        float g[N];                                  // the partners' channels
+        if (INTERLEAVED) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) f[e] = __fmul_rn(__fmul_rn(f[e], r), w[e]);
+            for (int e = 0; e < P; ++e) { g[2 * e] = f[2 * e + 1]; g[2 * e + 1] = f[2 * e]; }
+        } else if (half > 0) {                       // the same for every lane of the warp
+            const int from = peer + sub * LPR;
+            const uint4 o = make_uint4(__shfl_sync(0xffffffffu, raw[u].x, from), __shfl_sync(0xffffffffu, raw[u].y, from),
+                                       __shfl_sync(0xffffffffu, raw[u].z, from), __shfl_sync(0xffffffffu, raw[u].w, from));
+            Vec<T>::unpack(o, g);
+        }
+        if (warp_all) {
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                float2 o = fmul2(make_float2(g[2 * e], g[2 * e + 1]), cb[e]);
+                o = fmul2(ffma2(make_float2(f[2 * e], f[2 * e + 1]), ca[e], o), rr);
+                f[2 * e] = o.x; f[2 * e + 1] = o.y;
+            }
         } else {
 #pragma unroll
-            for (int e = 0; e < N; ++e) f[e] = __fmul_rn(f[e], w[e]);
-        }
-        if (INTERLEAVED) {
-            if (rot) {
-#pragma unroll
-                for (int e = 0; e < A; ++e)
-                    if (a0 + e < half) {
-                        const float a = f[2 * e], q = f[2 * e + 1];
-                        f[2 * e] = __fmaf_rn(a, cs[e], -__fmul_rn(q, sn[e]));
-                        f[2 * e + 1] = __fmaf_rn(a, sn[e], __fmul_rn(q, cs[e]));
-                    }
-            }
-        } else if (half > 0) {                       // the same for every lane of the warp
-            const int shift = half / N;
-            const int peer = (rot ? (c < half ? li + shift : li - shift) : li) + sub * LPR;
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const float o = __shfl_sync(0xffffffffu, f[e], peer);
-                if (rot) f[e] = __fmaf_rn(f[e], cs[e], c < half ? -__fmul_rn(o, sn[e]) : __fmul_rn(o, sn[e]));
+            for (int e = 0; e < P; ++e) {
+                const float2 v = make_float2(f[2 * e], f[2 * e + 1]);
+                float2 o;
+                if (all || (INTERLEAVED && a0 + e < half))
+                    o = ffma2(v, ca[e], fmul2(make_float2(g[2 * e], g[2 * e + 1]), cb[e]));
+                else
+                    o = fmul2(v, make_float2(w[2 * e], w[2 * e + 1]));
+                o = fmul2(o, rr);
+                f[2 * e] = o.x; f[2 * e + 1] = o.y;
             }
         }
-        const int h = h0 + u * kRows;
-        if (has && h < sd.heads) *reinterpret_cast<uint4*>(y + h * sd.ys_h) = Vec<T>::pack(f);
+        if (has && h0 + u * kRows < sd.heads) *reinterpret_cast<uint4*>(to) = Vec<T>::pack(f);
     }
 }
 
@@ -217,60 +285,68 @@ __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// Any width, stride and alignment: one warp per row, lane l holds channels
-// l, l + 32, ...; a pair's other channel is read again (from L1).
+// Any width, stride and alignment: the same lanes, channels and order of
+// arithmetic as rope_kernel (an output does not depend on the layout), element
+// by element; a pair's other channel is read again (from L1).
 template <typename T>
-__global__ void __launch_bounds__(32 * kWarps) rope_any_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(32 * kWarps) rope_any_kernel(const __grid_constant__ RopeParams p, int lpr) {
     pdl_wait();
     pdl_open();
-    const int lane = threadIdx.x & 31;
-    const int heads = p.side[0].heads + p.side[1].heads;
-    const int block = blockIdx.x / heads;
-    int h = blockIdx.x - block * heads;
+    constexpr int N = Vec<T>::N;
+    const int lane = threadIdx.x & 31, li = lane & (lpr - 1), sub = lane / lpr;
+    const int chunks = p.side[0].chunks + p.side[1].chunks;
+    const int block = blockIdx.x / chunks;
+    int chunk = blockIdx.x - block * chunks;
     const int64_t s = (int64_t)block * kWarps + (threadIdx.x >> 5);
     if (s >= p.tokens) return;
     const int64_t b = blockIdx.y;
-    const int which = h >= p.side[0].heads;
+    const int which = chunk >= p.side[0].chunks;
     const RopeSide& sd = p.side[which];
-    if (which) h -= p.side[0].heads;
+    if (which) chunk -= p.side[0].chunks;
+    const int h = chunk * (32 / lpr) + sub;
+    const bool row = h < sd.heads;
     const T* x = static_cast<const T*>(sd.x) + b * sd.xs_b + h * sd.xs_h + s * sd.xs_s;
     T* y = static_cast<T*>(sd.y) + b * sd.ys_b + h * sd.ys_h + s * sd.ys_s;
     const int half = s < p.rows ? p.half : 0;
-    float f[4], o[4];
-    float ss = 0.0f;
+    float f[N], g[N];
+    float s2[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = lane + 32 * i;
-        f[i] = c < p.d ? as_float(x[c]) : 0.0f;
-        ss = __fmaf_rn(f[i], f[i], ss);
-        o[i] = 0.0f;
-        if (c < 2 * half) o[i] = as_float(x[p.interleaved ? c ^ 1 : (c < half ? c + half : c - half)]);
+    for (int e = 0; e < N; ++e) {
+        const int c = li * N + e;
+        const bool in = row && c < p.d;
+        f[e] = in ? as_float(x[c]) : 0.0f;
+        g[e] = in && c < 2 * half ? as_float(x[p.interleaved ? c ^ 1 : (c < half ? c + half : c - half)]) : 0.0f;
+        s2[e & 1] = __fmaf_rn(f[e], f[e], s2[e & 1]);
     }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-    const float r = p.norm ? __frsqrt_rn(__fmaf_rn(ss, 1.0f / (float)p.d, p.eps)) : 1.0f;
+    float r = 1.0f;
+    if (p.norm) {
+        float ss = __fadd_rn(s2[0], s2[1]);
+        for (int o = lpr / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        r = rsqrtf(__fmaf_rn(ss, 1.0f / (float)p.d, p.eps));
+    }
     const int64_t t = b * p.ts_b + s * p.ts_s;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = lane + 32 * i;
-        if (c >= p.d) continue;
-        f[i] = __fmul_rn(f[i], r);
-        if (sd.w) f[i] = __fmul_rn(f[i], load_as_float(sd.w, c, sd.w_dtype));
+    for (int e = 0; e < N; ++e) {
+        const int c = li * N + e;
+        if (!row || c >= p.d) continue;
+        const float w = sd.w ? load_as_float(sd.w, c, sd.w_dtype) : 1.0f;
         if (c < 2 * half) {
             const int peer = p.interleaved ? c ^ 1 : (c < half ? c + half : c - half);
             const bool first = p.interleaved ? !(c & 1) : c < half;
             const int a = p.interleaved ? c >> 1 : (c < half ? c : c - half);
-            float q = __fmul_rn(o[i], r);
-            if (sd.w) q = __fmul_rn(q, load_as_float(sd.w, peer, sd.w_dtype));
-            const float qs = __fmul_rn(q, __ldg(p.sin + t + a));
-            f[i] = __fmaf_rn(f[i], __ldg(p.cos + t + a), first ? -qs : qs);
+            const float wp = sd.w ? load_as_float(sd.w, peer, sd.w_dtype) : 1.0f;
+            const float ws = __fmul_rn(wp, __ldg(p.sin + t + a));
+            f[e] = __fmaf_rn(f[e], __fmul_rn(w, __ldg(p.cos + t + a)), __fmul_rn(g[e], first ? -ws : ws));
+        } else {
+            f[e] = __fmul_rn(f[e], w);
         }
+        f[e] = __fmul_rn(f[e], r);
     }
-    __syncwarp();                       // every lane has read the row: it may be the output
+    __syncwarp();                       // every lane has read its row: it may be the output
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = lane + 32 * i;
-        if (c < p.d) y[c] = from_float<T>(f[i]);
+    for (int e = 0; e < N; ++e) {
+        const int c = li * N + e;
+        if (row && c < p.d) y[c] = from_float<T>(f[e]);
     }
 }
 
@@ -287,12 +363,15 @@ cudaError_t launch_vec(RopeParams& p, int64_t batch, cudaStream_t st) {
 template <typename T>
 int launch(RopeParams& p, int64_t batch, bool vec, cudaStream_t st) {
     constexpr int N = Vec<T>::N;
+    const int lanes = (p.d + N - 1) / N;
     if (!vec) {
-        const int64_t blocks = (p.tokens + kWarps - 1) / kWarps * (p.side[0].heads + p.side[1].heads);
-        VCB_CUDA(launch_pdl(rope_any_kernel<T>, dim3((unsigned)blocks, (unsigned)batch), dim3(32 * kWarps), 0, st, p));
+        int lpr = 4;
+        while (lpr < lanes) lpr *= 2;
+        for (RopeSide& s : p.side) s.chunks = (s.heads + 32 / lpr - 1) / (32 / lpr);
+        const int64_t blocks = (p.tokens + kWarps - 1) / kWarps * (p.side[0].chunks + p.side[1].chunks);
+        VCB_CUDA(launch_pdl(rope_any_kernel<T>, dim3((unsigned)blocks, (unsigned)batch), dim3(32 * kWarps), 0, st, p, lpr));
         return VCB_OK;
     }
-    const int lanes = (p.d + N - 1) / N;
     if (lanes <= 4) VCB_CUDA((launch_vec<T, 4>(p, batch, st)));
     else if (lanes <= 8) VCB_CUDA((launch_vec<T, 8>(p, batch, st)));
     else if (lanes <= 16 || N > 4) VCB_CUDA((launch_vec<T, 16>(p, batch, st)));
@@ -315,6 +394,7 @@ int rope_run(const vcb_qk_norm_rope_args* a, cudaStream_t st) {
         s.y = i ? a->k_out : a->q_out;
         s.w = i ? a->k_weight : a->q_weight;
         s.w_dtype = a->weight_dtype;
+        s.w_vec = aligned(s.w, 16);
         s.heads = (int)(i ? a->k_heads : a->q_heads);
         const int64_t* xs = i ? a->k_stride : a->q_stride;
         const int64_t* ys = i ? a->k_out_stride : a->q_out_stride;

@@ -671,26 +671,40 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
     pdl_open();
     __shared__ float qrow[8][128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t r = (int64_t)blockIdx.x * 8 + warp;
-    const int item = p.whole + (int)(r / (128 * NQ));
+    // a row of the items behind the whole ones; with one query tile per head an
+    // item has sq rows only
+    const int per = p.q_tiles == 1 ? (int)p.sq : 128 * NQ;
+    const int64_t n = (int64_t)blockIdx.x * 8 + warp;
+    const int cut = (int)(n / per), in = (int)(n - (int64_t)cut * per), item = p.whole + cut;
+    if ((int64_t)cut * (128 * NQ) >= p.part_rows) return;
     const int64_t bh = item / p.q_tiles, b = bh / p.heads, h = bh - b * p.heads;
-    const int64_t i = (int64_t)(p.q_tiles - 1 - item % p.q_tiles) * (128 * NQ) + r % (128 * NQ);
+    const int64_t i = (int64_t)(p.q_tiles - 1 - item % p.q_tiles) * (128 * NQ) + in;
     if (i >= p.sq) return;
-    const int64_t rows = p.part_rows;
+    const int64_t rows = p.part_rows, r = (int64_t)cut * (128 * NQ) + in;
     const int64_t len = keys_of(p, b);
     const Seen s = seen_at(p, i + (p.has_offset ? p.q_offset : len - p.sq), len);
     const bool sees = s.sink > 0 || s.hi > s.lo;
     constexpr int kPer = HD / 32;                                // channels per lane
-    float acc[kPer] = {}, den = 0.0f, top = -INFINITY;
-    for (int q = 0; q < p.splits; ++q) top = fmaxf(top, p.part_ml[q * rows + r].x);
-    for (int q = 0; q < p.splits; ++q) {
-        const float2 ml = p.part_ml[q * rows + r];
-        if (ml.x == -INFINITY && ml.y == 0.0f) continue;         // no key of this part is seen
-        const float w = ex2_ftz(ml.x - top);
-        den = __fmaf_rn(ml.y, w, den);
+    // lane q holds part q's maximum and weight (32 parts at most)
+    const float2 ml = lane < p.splits ? p.part_ml[lane * rows + r] : make_float2(-INFINITY, 0.0f);
+    float top = ml.x;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e)
-            acc[e] = __fmaf_rn(p.part[(q * rows + r) * HD + lane + 32 * e], w, acc[e]);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // a part that sees no key of the row has no weight, whatever its sums hold
+    const bool has = !(ml.x == -INFINITY && ml.y == 0.0f);
+    const float mine = has ? ex2_ftz(ml.x - top) : 0.0f;
+    const unsigned parts = __ballot_sync(0xffffffffu, has);
+    float acc[kPer] = {}, den = 0.0f;
+#pragma unroll 8
+    for (int q = 0; q < p.splits; ++q) {
+        const float w = __shfl_sync(0xffffffffu, mine, q), d = __shfl_sync(0xffffffffu, ml.y, q);
+        const bool on = parts >> q & 1u;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            const float o = on ? p.part[(q * rows + r) * HD + lane + 32 * e] : 0.0f;
+            acc[e] = __fmaf_rn(o, w, acc[e]);
+        }
+        den = __fmaf_rn(d, w, den);
     }
     T* out = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + i * p.os[2];
     bool bad = false;
@@ -787,7 +801,10 @@ template <typename T, int HD, int NQ> int launch(const WinParams& p, const WinPl
     const int64_t cut = r.items - r.whole;
     VCB_CUDA(launch_pdl(window_kernel<T, HD, NQ>, dim3((unsigned)(r.whole + cut * r.splits)), dim3(L::kThreads), L::kSmem,
                         st, p));
-    if (cut) VCB_CUDA(launch_pdl(window_join_kernel<T, HD, NQ>, dim3((unsigned)(cut * 16 * NQ)), dim3(256), 0, st, p));
+    if (cut) {
+        const int64_t rows = cut * (p.q_tiles == 1 ? p.sq : 128 * NQ);
+        VCB_CUDA(launch_pdl(window_join_kernel<T, HD, NQ>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p));
+    }
     return VCB_OK;
 }
 template <typename T> int launch_any(const WinParams& p, const WinPlan& r, cudaStream_t st) {
