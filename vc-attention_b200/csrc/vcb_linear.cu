@@ -252,23 +252,48 @@ __device__ __forceinline__ float gelu_erf(float y) {
     return y * (y < 0.0f ? e : 1.0f - e);
 }
 
-__device__ __forceinline__ float act_of(int kind, float y) {
-    switch (kind) {
-        case VCB_ACT_SILU: return __fdividef(y, 1.0f + __expf(-y));
-        case VCB_ACT_GELU: return gelu_erf(y);
-        // 0.5 y (1 + tanh u) = y / (1 + exp(-2 u)), u = sqrt(2/pi) (y + 0.044715 y^3)
-        case VCB_ACT_GELU_TANH: {
-            const float u2 = 1.5957691216057308f * y * __fmaf_rn(0.044715f * y, y, 1.0f);
-            return __fdividef(y, 1.0f + __expf(-u2));
-        }
-        case VCB_ACT_RELU: return fmax_nan(y, 0.0f);
-        default: return y;
+__device__ __forceinline__ float silu(float y) { return __fdividef(y, 1.0f + __expf(-y)); }
+// 0.5 y (1 + tanh u) = y / (1 + exp(-2 u)), u = sqrt(2/pi) (y + 0.044715 y^3)
+__device__ __forceinline__ float gelu_tanh(float y) {
+    return __fdividef(y, 1.0f + __expf(-1.5957691216057308f * y * __fmaf_rn(0.044715f * y, y, 1.0f)));
+}
+
+template <int N> __device__ __forceinline__ void activate(int kind, float (&f)[N]) {
+    switch (kind) {                     // the same for all threads
+        case VCB_ACT_SILU:
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = silu(f[e]);
+            break;
+        case VCB_ACT_GELU:
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = gelu_erf(f[e]);
+            break;
+        case VCB_ACT_GELU_TANH:
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = gelu_tanh(f[e]);
+            break;
+        case VCB_ACT_RELU:
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = fmax_nan(f[e], 0.0f);
+            break;
+        default: break;
     }
 }
 
-// Eight consecutive values of a bias or gate row as floats (16-byte aligned).
-__device__ __forceinline__ void load8_any(const void* p, int64_t i, int dtype, float* o) {
-    if (dtype == VCB_F32) {
+__device__ __forceinline__ float load1_any(const void* p, int64_t i, int dtype) {
+    if (dtype == VCB_F32) return static_cast<const float*>(p)[i];
+    if (dtype == VCB_F16) return __half2float(static_cast<const __half*>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+// Eight consecutive values of a bias or gate row as floats: 16-byte aligned
+// (VEC), or one by one and none at or behind `valid`.
+template <bool VEC>
+__device__ __forceinline__ void load8_any(const void* p, int64_t i, int dtype, int valid, float* o) {
+    if (!VEC) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = e < valid ? load1_any(p, i + e, dtype) : 0.0f;
+    } else if (dtype == VCB_F32) {
         const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
         const float4 a = f[0], b = f[1];
         o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w; o[4] = b.x; o[5] = b.y; o[6] = b.z; o[7] = b.w;
@@ -297,64 +322,72 @@ __device__ __forceinline__ RowAt row_at(const LinParams& p, int64_t b, int64_t r
     return {b * p.ys_b + s * p.ys_s, b * p.gs_b + s * p.gs_s, b * p.rs_b + s * p.rs_s, row < p.rows};
 }
 
-// Four rows of a 32 x 32 block, eight columns n .. n + 7 of each (16-byte runs):
-// all reads of the gate and the residual come before the first store, since
-// the output may be the residual itself and would hold them back.
-template <typename T>
-__device__ __forceinline__ void finish_rows(const LinParams& p, float (&f)[4][8], const float* bias, int n,
-                                            const RowAt (&at)[4], int h, int64_t col) {
-    uint4 res[4];
-    if (p.residual) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (at[i].live) res[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.residual) + at[i].r + n);
-    }
+// Bias, activation and gate on four rows of a 32 x 32 block, eight columns
+// n .. n + 7 of each (fewer at the last column when not VEC).
+template <bool VEC>
+__device__ __forceinline__ void finish_rows(const LinParams& p, float (&f)[4][8], int n, const RowAt (&at)[4]) {
+    float bias[8];
+    if (p.bias) load8_any<VEC>(p.bias, n, p.bias_dtype, p.n - n, bias);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float gate[8];
-        if (p.gate && at[i].live) load8_any(p.gate, at[i].g + n, p.gate_dtype, gate);
+        if (p.gate && at[i].live) load8_any<VEC>(p.gate, at[i].g + n, p.gate_dtype, p.n - n, gate);
         if (p.bias) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[i][e] = __fadd_rn(f[i][e], bias[e]);
         }
-        if (p.activation != VCB_ACT_NONE) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[i][e] = act_of(p.activation, f[i][e]);
-        }
-        if (p.gate) {
+        activate(p.activation, f[i]);
+        if (p.gate && at[i].live) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[i][e] = __fmul_rn(f[i][e], gate[e]);
         }
-        if (p.residual) {
-            const uint32_t w[4] = {res[i].x, res[i].y, res[i].z, res[i].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 q = F16<T>::both(w[e]);
-                f[i][2 * e] = __fadd_rn(f[i][2 * e], q.x);
-                f[i][2 * e + 1] = __fadd_rn(f[i][2 * e + 1], q.y);
-            }
-        }
     }
-    T* y = static_cast<T*>(p.y) + h * p.ys_h + col;
+}
+template <typename T> __device__ __forceinline__ void add_residual(float (&f)[8], const uint4& u) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (at[i].live)
-            *reinterpret_cast<uint4*>(y + at[i].y) =
-                make_uint4(F16<T>::two(f[i][0], f[i][1]), F16<T>::two(f[i][2], f[i][3]), F16<T>::two(f[i][4], f[i][5]),
-                           F16<T>::two(f[i][6], f[i][7]));
+    for (int e = 0; e < 4; ++e) {
+        const float2 q = F16<T>::both(w[e]);
+        f[2 * e] = __fadd_rn(f[2 * e], q.x);
+        f[2 * e + 1] = __fadd_rn(f[2 * e + 1], q.y);
+    }
+}
+template <typename T> __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+    return make_uint4(F16<T>::two(f[0], f[1]), F16<T>::two(f[2], f[3]), F16<T>::two(f[4], f[5]), F16<T>::two(f[6], f[7]));
 }
 
-__device__ __forceinline__ float load1_any(const void* p, int64_t i, int dtype) {
-    if (dtype == VCB_F32) return static_cast<const float*>(p)[i];
-    if (dtype == VCB_F16) return __half2float(static_cast<const __half*>(p)[i]);
-    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+// fn(r, y or residual offset of the row) for the live rows among 32 from `row` on
+template <bool Y, typename Fn>
+__device__ __forceinline__ void each_row(const LinParams& p, int64_t b, int64_t row, Fn&& fn) {
+    const int live = (int)min((int64_t)32, p.rows - row);
+    RowAt at = row_at(p, b, row);
+    int64_t off = Y ? at.y : at.r;
+    const int64_t step = Y ? p.ys_s : p.rs_s;
+    uint32_t s = p.collapsed ? (uint32_t)row % (uint32_t)p.tokens : 0;
+    if (live == 32 && (!p.collapsed || s + 32 <= (uint32_t)p.tokens)) {        // evenly spaced
+#pragma unroll 8
+        for (int r = 0; r < 32; ++r) fn(r, off + r * step);
+        return;
+    }
+#pragma unroll 1
+    for (int r = 0; r < live; ++r) {
+        fn(r, off);
+        off += step;
+        if (p.collapsed && ++s == (uint32_t)p.tokens) {     // the next row begins a batch entry
+            s = 0;
+            at = row_at(p, b, row + r + 1);
+            off = Y ? at.y : at.r;
+        }
+    }
 }
 
 // One sum's epilogue, for outputs off the 16-byte grid and the small kernels:
 // column n = head h, channel col.
 template <typename T>
 __device__ __forceinline__ float finish1(const LinParams& p, float f, float bias, int n, const RowAt& at, float residual) {
-    f = act_of(p.activation, __fadd_rn(f, bias));
+    float v[1] = {__fadd_rn(f, bias)};
+    activate(p.activation, v);
+    f = v[0];
     if (p.gate) f = __fmul_rn(f, load1_any(p.gate, at.g + n, p.gate_dtype));
     return p.residual ? __fadd_rn(f, residual) : f;
 }
@@ -410,47 +443,60 @@ __device__ void lin_epilogue(const LinParams& p, uint8_t* smem, const LinBars& B
                     to[0] = stage[row * 8 + ((q8 >> 2) ^ (row & 7))];
                     to[1] = stage[row * 8 + (((q8 >> 2) + 1) ^ (row & 7))];
                 }
-            } else if (p.vec) {
+            } else {
                 const int n = n0 + q8;
-                if (n < p.n) {
-                    float bias[8], f[4][8];
-                    if (p.bias) load8_any(p.bias, n, p.bias_dtype, bias);
+                float f[4][8];
+                uint4 res[4];
+                if (p.vec && p.residual && n < p.n) {
+                    // read before the first store, since the output may be the residual itself
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (at[i].live) res[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.residual) + at[i].r + n);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = r0 + 8 * i;
+                    const float4 a = stage[row * 8 + ((q8 >> 2) ^ (row & 7))];
+                    const float4 d = stage[row * 8 + (((q8 >> 2) + 1) ^ (row & 7))];
+                    f[i][0] = a.x; f[i][1] = a.y; f[i][2] = a.z; f[i][3] = a.w;
+                    f[i][4] = d.x; f[i][5] = d.y; f[i][6] = d.z; f[i][7] = d.w;
+                }
+                if (p.vec) {
+                    if (n < p.n) {
+                        finish_rows<true>(p, f, n, at);
+                        const int h = n / p.n_head;
+                        T* y = static_cast<T*>(p.y) + h * p.ys_h + (n - h * p.n_head);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (p.residual) add_residual<T>(f[i], res[i]);
+                            if (at[i].live) *reinterpret_cast<uint4*>(y + at[i].y) = pack8<T>(f[i]);
+                        }
+                    }
+                } else {
+                    // Off the 16-byte grid: the residual comes in and y goes out one
+                    // column per lane (64-byte runs), through the same block.
+                    uint16_t* block = reinterpret_cast<uint16_t*>(stage);       // [32 rows][32 columns]
+                    const int nl = n0 + lane;
+                    const bool in = nl < p.n;
+                    __syncwarp();
+                    if (p.residual) {
+                        const uint16_t* src = static_cast<const uint16_t*>(p.residual) + nl;
+                        each_row<false>(p, tb, row0 - r0, [&](int r, int64_t off) { block[r * 32 + lane] = in ? src[off] : 0; });
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) res[i] = *reinterpret_cast<const uint4*>(block + (r0 + 8 * i) * 32 + q8);
+                    }
+                    finish_rows<false>(p, f, n, at);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int row = r0 + 8 * i;
-                        const float4 a = stage[row * 8 + ((q8 >> 2) ^ (row & 7))];
-                        const float4 d = stage[row * 8 + (((q8 >> 2) + 1) ^ (row & 7))];
-                        f[i][0] = a.x; f[i][1] = a.y; f[i][2] = a.z; f[i][3] = a.w;
-                        f[i][4] = d.x; f[i][5] = d.y; f[i][6] = d.z; f[i][7] = d.w;
+                        if (p.residual) add_residual<T>(f[i], res[i]);
+                        *reinterpret_cast<uint4*>(block + (r0 + 8 * i) * 32 + q8) = pack8<T>(f[i]);
                     }
-                    const int h = n / p.n_head;
-                    finish_rows<T>(p, f, bias, n, at, h, n - h * p.n_head);
-                }
-            } else {
-                // one column per lane: 64-byte runs whatever the alignment, eight
-                // rows' reads in flight
-                const int n = n0 + lane;
-                const bool in = n < p.n;
-                const float bias = p.bias && in ? load1_any(p.bias, n, p.bias_dtype) : 0.0f;
-                const int h = n / p.n_head, col = n - h * p.n_head;
-                const float* one = reinterpret_cast<const float*>(stage);
-#pragma unroll 1
-                for (int r8 = 0; r8 < 32; r8 += 8) {
-                    RowAt q[8];
-                    float res[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        q[i] = row_at(p, tb, row0 - r0 + r8 + i);
-                        res[i] = p.residual && in && q[i].live
-                                     ? F16<T>::to(static_cast<const T*>(p.residual)[q[i].r + n]) : 0.0f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int row = r8 + i;
-                        const float f = one[row * 32 + (((lane >> 2) ^ (row & 7)) << 2) + (lane & 3)];
-                        if (in && q[i].live)
-                            static_cast<T*>(p.y)[q[i].y + h * p.ys_h + col] =
-                                F16<T>::one(finish1<T>(p, f, bias, n, q[i], res[i]));
+                    __syncwarp();
+                    if (in) {
+                        const int h = nl / p.n_head;
+                        uint16_t* dst = static_cast<uint16_t*>(p.y) + h * p.ys_h + (nl - h * p.n_head);
+                        each_row<true>(p, tb, row0 - r0, [&](int r, int64_t off) { dst[off] = block[r * 32 + lane]; });
                     }
                 }
             }
