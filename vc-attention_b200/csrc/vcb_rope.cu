@@ -197,11 +197,19 @@ __global__ void __launch_bounds__(32 * kWarps, 4) rope_kernel(const __grid_const
     const bool all = rot && a0 + A <= half;          // every channel of this lane turns
     const int shift = half / (INTERLEAVED ? 1 : N);  // half-split: lanes between partners
     const int peer = INTERLEAVED || !rot ? li : (low ? li + shift : li - shift);
-    float w[N];
-    float2 ca[P], cb[P];                             // A and B of channel pairs 2e, 2e + 1
+    // A and B of channel pairs 2e, 2e + 1; where nothing turns A = w and B = 0, and
+    // the partner is taken as 0 too (0 times a NaN or infinity would not be)
+    float2 ca[P], cb[P];
     {
-        float cs[A], sn[A], wp[N];
+        float w[N], cs[A], sn[A], wp[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = 1.0f;
         if (has) load_weights<N>(sd, c, w);
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+            ca[e] = make_float2(w[2 * e], w[2 * e + 1]);
+            cb[e] = make_float2(0.0f, 0.0f);
+        }
         if (rot) {
             const int64_t t = b * p.ts_b + s * p.ts_s;
             load_table<A>(p.cos + t, a0, half, p.table_vec, cs);
@@ -210,6 +218,7 @@ __global__ void __launch_bounds__(32 * kWarps, 4) rope_kernel(const __grid_const
 #pragma unroll
             for (int e = 0; e < P; ++e) {
                 if (INTERLEAVED) {
+                    if (a0 + e >= half) break;
                     ca[e] = make_float2(__fmul_rn(w[2 * e], cs[e]), __fmul_rn(w[2 * e + 1], cs[e]));
                     cb[e] = make_float2(-__fmul_rn(w[2 * e + 1], sn[e]), __fmul_rn(w[2 * e], sn[e]));
                 } else {
@@ -247,31 +256,23 @@ __global__ void __launch_bounds__(32 * kWarps, 4) rope_kernel(const __grid_const
         if (INTERLEAVED) {
 #pragma unroll
             for (int e = 0; e < P; ++e) { g[2 * e] = f[2 * e + 1]; g[2 * e + 1] = f[2 * e]; }
-        } else if (half > 0) {                       // the same for every lane of the warp
-            const int from = peer + sub * LPR;
-            const uint4 o = make_uint4(__shfl_sync(0xffffffffu, raw[u].x, from), __shfl_sync(0xffffffffu, raw[u].y, from),
-                                       __shfl_sync(0xffffffffu, raw[u].z, from), __shfl_sync(0xffffffffu, raw[u].w, from));
-            Vec<T>::unpack(o, g);
-        }
-        if (warp_all) {
+            if (!warp_all) {
 #pragma unroll
-            for (int e = 0; e < P; ++e) {
-                float2 o = fmul2(make_float2(g[2 * e], g[2 * e + 1]), cb[e]);
-                o = fmul2(ffma2(make_float2(f[2 * e], f[2 * e + 1]), ca[e], o), rr);
-                f[2 * e] = o.x; f[2 * e + 1] = o.y;
+                for (int e = 0; e < P; ++e)
+                    if (a0 + e >= half) g[2 * e] = g[2 * e + 1] = 0.0f;
             }
         } else {
+            const int from = peer + sub * LPR;
+            uint4 o = make_uint4(__shfl_sync(0xffffffffu, raw[u].x, from), __shfl_sync(0xffffffffu, raw[u].y, from),
+                                 __shfl_sync(0xffffffffu, raw[u].z, from), __shfl_sync(0xffffffffu, raw[u].w, from));
+            if (!rot) o = make_uint4(0, 0, 0, 0);
+            Vec<T>::unpack(o, g);
+        }
 #pragma unroll
-            for (int e = 0; e < P; ++e) {
-                const float2 v = make_float2(f[2 * e], f[2 * e + 1]);
-                float2 o;
-                if (all || (INTERLEAVED && a0 + e < half))
-                    o = ffma2(v, ca[e], fmul2(make_float2(g[2 * e], g[2 * e + 1]), cb[e]));
-                else
-                    o = fmul2(v, make_float2(w[2 * e], w[2 * e + 1]));
-                o = fmul2(o, rr);
-                f[2 * e] = o.x; f[2 * e + 1] = o.y;
-            }
+        for (int e = 0; e < P; ++e) {
+            float2 o = fmul2(make_float2(g[2 * e], g[2 * e + 1]), cb[e]);
+            o = fmul2(ffma2(make_float2(f[2 * e], f[2 * e + 1]), ca[e], o), rr);
+            f[2 * e] = o.x; f[2 * e + 1] = o.y;
         }
         if (has && h0 + u * kRows < sd.heads) *reinterpret_cast<uint4*>(to) = Vec<T>::pack(f);
     }

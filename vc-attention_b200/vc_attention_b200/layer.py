@@ -190,7 +190,7 @@ def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, h
         return linear(x, weight, bias, activation=activation, gate=gate, residual=residual, heads_in=heads_in,
                       heads_out=heads_out, out=out, status=status)
     if out is None:
-        out = torch.empty(plan.shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(plan.shape)
     plan.call(x.device, x=x.data_ptr(), w=weight.data_ptr(), y=out.data_ptr(), bias=_ptr(bias), gate=_ptr(gate),
               residual=_ptr(residual), status=_ptr(status))
     return out
@@ -307,8 +307,8 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, *, eps=
                                               for t in (q, k, q_weight, k_weight, cos, sin))
         return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps=eps, interleaved=interleaved, out=out)
     if out is None:
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
         qo, ko = out
     plan.call(q.device, q=q.data_ptr(), k=k.data_ptr(), q_out=qo.data_ptr(), k_out=ko.data_ptr(),

@@ -55,7 +55,7 @@ def window_attention(q, k, v, *, window=(None, None), sinks=0, causal=False, q_o
         return window_attention(q, k, v, window=window, sinks=sinks, causal=causal, q_offset=q_offset, kv_lens=kv_lens,
                                 scale=scale, out=out, status=status)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     plan.call(q.device, q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), kv_lens=_ptr(kv_lens),
               status=_ptr(status))
     return out
