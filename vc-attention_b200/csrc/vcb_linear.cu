@@ -158,8 +158,6 @@ template <int BN>
 __device__ void lin_producer(const LinParams& p, uint8_t* smem, const LinBars& B, const Waiter& wait, uint32_t rank,
                              int c, int ncl) {
     using L = Tile<BN>;
-    prefetch_tmap(&p.tm_x);
-    prefetch_tmap(&p.tm_w);
     const uint32_t lead = peer_addr(B.full, 0);
     uint32_t g = 0;
     bool ok = true;
@@ -413,12 +411,29 @@ __device__ void lin_epilogue(const LinParams& p, uint8_t* smem, const LinBars& B
         for (int i = 0; i < 4; ++i) at[i] = row_at(p, tb, row0 + 8 * i);
         float* part = wk.slot < 0 ? nullptr
                                   : p.part + ((int64_t)wk.slot * 256 + rank * 128 + quarter * 32 + r0) * BN +
-                                        side * kHalfCols + q8;
+                                        side * kHalfCols + 4 * (lane & 3);
         const uint32_t buf = li & 1;
+        // the residual's runs of the next block, a block ahead (no other block's
+        // output touches them, so y may be the residual itself)
+        const bool ahead = p.vec && p.residual && !part;
+        uint4 next[4];
+        auto fetch = [&](int ch) {
+            const int n = nt * BN + side * kHalfCols + ch * 32 + q8;
+            if (ahead && n < p.n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (at[i].live) next[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.residual) + at[i].r + n);
+            }
+        };
+        fetch(0);
         if (!wait.parked(&B.acc_full[buf], (li >> 1) & 1)) return;
         tc_fence_after();
 #pragma unroll 1
         for (int ch = 0; ch < kChunks; ++ch) {
+            uint4 res[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) res[i] = next[i];
+            if (ch + 1 < kChunks) fetch(ch + 1);
             uint32_t r[32];
             tmem_ld32_at<0>(trow + buf * BN + ch * 32, r);
             tmem_wait_ld();
@@ -440,19 +455,12 @@ __device__ void lin_epilogue(const LinParams& p, uint8_t* smem, const LinBars& B
                     const int row = r0 + 8 * i;
                     if (!at[i].live) continue;
                     float4* to = reinterpret_cast<float4*>(part + (int64_t)(8 * i) * BN + ch * 32);
-                    to[0] = stage[row * 8 + ((q8 >> 2) ^ (row & 7))];
-                    to[1] = stage[row * 8 + (((q8 >> 2) + 1) ^ (row & 7))];
+                    to[0] = stage[row * 8 + ((lane & 3) ^ (row & 7))];             // 64-byte runs of a row
+                    to[4] = stage[row * 8 + (((lane & 3) + 4) ^ (row & 7))];
                 }
             } else {
                 const int n = n0 + q8;
                 float f[4][8];
-                uint4 res[4];
-                if (p.vec && p.residual && n < p.n) {
-                    // read before the first store, since the output may be the residual itself
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (at[i].live) res[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.residual) + at[i].r + n);
-                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int row = r0 + 8 * i;
@@ -522,6 +530,10 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_kernel(const __grid_con
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int c = (int)(blockIdx.x >> 1), ncl = (int)(gridDim.x >> 1);
+    if (threadIdx.x == 32) {             // while the barriers are set up
+        prefetch_tmap(&p.tm_x);
+        prefetch_tmap(&p.tm_w);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < L::kStages; ++s) {
             mbar_init(&B.full[s], 1);
@@ -722,9 +734,7 @@ template <typename T, int MT, int NT> int launch_few(const FewParams& p, cudaStr
     return VCB_OK;
 }
 template <typename T> int launch_few_any(const FewParams& p, cudaStream_t st) {
-    if (p.l.rows <= 8) return launch_few<T, 1, 1>(p, st);
-    if (p.l.rows <= 16) return launch_few<T, 1, 2>(p, st);
-    return launch_few<T, 2, 4>(p, st);
+    return p.l.rows <= 8 ? launch_few<T, 1, 1>(p, st) : launch_few<T, 1, 2>(p, st);
 }
 
 template <typename T, int BN>
@@ -762,7 +772,7 @@ int launch_tiles(const LinParams& p, int grid_pairs, cudaStream_t st) {
 }
 
 // Up to this many rows of x the product streams w through linear_few_kernel.
-constexpr int kFewRows = 32;
+constexpr int kFewRows = 16;
 
 struct LinPlan {
     bool pack_x, pack_w;

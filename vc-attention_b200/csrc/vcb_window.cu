@@ -324,9 +324,6 @@ __device__ __forceinline__ void mma_commit_elected(uint64_t* bar) {
 
 template <typename L>
 __device__ void win_producer(const WinParams& p, const WinItem& it, int fix, uint8_t* smem, const WinBars& B, volatile int* abort) {
-    prefetch_tmap(&p.tm_q);
-    prefetch_tmap(&p.tm_k);
-    prefetch_tmap(&p.tm_v);
     mbar_arrive_expect_tx(B.q_full, it.nq * L::kBytes);
     for (int w = 0; w < it.nq; ++w)
         for (int x = 0; x < L::kBoxes; ++x)
@@ -605,6 +602,11 @@ __global__ void __launch_bounds__(WinTile<HD, NQ>::kThreads, WinTile<HD, NQ>::kC
     volatile int* abort = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;      // warp: uniform
     const WinItem it = win_item<NQ>(p);
+    if (threadIdx.x == 32) {             // while the barriers are set up
+        prefetch_tmap(&p.tm_q);
+        prefetch_tmap(&p.tm_k);
+        prefetch_tmap(&p.tm_v);
+    }
     if (threadIdx.x == 0) {
         mbar_init(B.q_full, 1);
         for (int s = 0; s < L::kStages; ++s) {
