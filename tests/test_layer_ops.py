@@ -321,3 +321,60 @@ def test_rope_non_finite_rows_and_zero_rows():
         bad[0, 0, 8, 0] = float("inf")
         got, _ = qk_norm_rope(bad, q, None, None, cos[:8], sin[:8], eps=None)
         assert got[0, 0, 8, 0] == float("inf") and got[0, 0, 8, 1:].isfinite().all()
+
+
+def test_offsets_past_32_bits():
+    """Outputs, inputs and caches of more than 2^31 elements: the last rows are
+    what the same rows give alone."""
+    from vc_attention_b200 import linear, qk_norm_rope, window_attention
+    g = _gen(21)
+    s, k, n = 135000, 64, 16000                      # 2.16e9 outputs
+    x, w = _randn((1, s, k), BF16, g), _randn((n, k), BF16, g)
+    y = linear(x, w)
+    for lo in (0, s // 2, s - 300):
+        assert torch.equal(y[:, lo:lo + 300], linear(x[:, lo:lo + 300].contiguous(), w))
+    heads = linear(x, w, heads_out=125)
+    assert torch.equal(heads[:, 124, -300:], y[:, -300:, -128:])
+    del heads
+    back = linear(y[:, -40:], w.t().contiguous())    # rows behind 2^31 elements as input
+    assert torch.equal(back, linear(y[:, -40:].clone(), w.t().contiguous()))
+    del y, back
+    b, h, s, d = 1, 40, 425000, 128                  # 2.18e9 elements
+    big = torch.empty((b, h, s, d), device="cuda", dtype=BF16).normal_(generator=g)
+    cos, sin = _tables(s, d // 2, g)
+    q, ko = qk_norm_rope(big, big, None, None, cos, sin)
+    assert torch.equal(q, ko)
+    tail, _ = qk_norm_rope(big[:, :, -100:], big[:, :, -100:], None, None, cos[-100:], sin[-100:])
+    assert torch.equal(q[:, :, -100:], tail)
+    del ko
+    got = window_attention(q[:, :, -3:], q, big, window=(500, 0), causal=True)
+    near = slice(s - 640, s)
+    want = window_attention(q[:, :, -3:], q[:, :, near].contiguous(), big[:, :, near].contiguous(), window=(500, 0),
+                            causal=True)
+    assert (got.double() - want.double()).abs().max() <= 2.0 ** -7 * big[:, :, near].abs().max().double()
+
+
+def test_calls_of_one_shape_from_two_threads():
+    """The checked arguments of a shape are shared; addresses are not."""
+    import threading
+
+    from vc_attention_b200 import linear
+    g = _gen(22)
+    x = [_randn((1, 40, 256), BF16, g) for _ in range(8)]
+    w = _randn((96, 256), BF16, g)
+    want = [linear(t, w) for t in x]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                if not torch.equal(linear(x[i], w), want[i]):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

@@ -67,6 +67,7 @@ TAB = _t(6, 8, dtype=torch.float32)
     ((_t(1, 1, 2, 130), _t(1, 1, 2, 130)), {}, "<= 128"),
     ((Q, Q), dict(eps=-1.0), "eps"),
     ((Q, Q), dict(eps=float("nan")), "eps"),
+    ((Q, Q), dict(eps=torch.tensor(1e-6)), "eps"),
     ((Q, Q, _t(15)), {}, "weights"),
     ((Q, Q, _t(16, dtype=torch.float16)), {}, "weights"),
     ((Q, Q, _t(16), _t(16, dtype=torch.float32)), {}, "share a dtype"),
@@ -160,6 +161,8 @@ W = _t(2, 3, 5, 16)
     ((W, W, W), dict(kv_lens=torch.zeros(3, dtype=torch.int32)), "kv_lens"),
     ((W, W, W), dict(scale=0.0), "scale"),
     ((W, W, W), dict(scale=float("inf")), "scale"),
+    ((W, W, W), dict(scale=torch.tensor(0.5)), "scale"),
+    ((W, W, W), dict(window=None), "window"),
     ((W, W, W), dict(out=W), "share memory"),
     ((W, W, W), dict(status=_t(2, dtype=torch.int32)), "status"),
     ((W, W, W), {}, "no CPU fallback"),

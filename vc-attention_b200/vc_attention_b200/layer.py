@@ -339,7 +339,7 @@ def _rope_plan(q, k, q_weight, k_weight, cos, sin, eps, interleaved, out):
     b, h, s, d = q.shape
     if d > 128:
         raise ValueError("qk_norm_rope supports head dimensions <= 128")
-    if eps is not None and not (math.isfinite(eps) and eps >= 0):
+    if eps is not None and not (isinstance(eps, (int, float)) and math.isfinite(eps) and eps >= 0):
         raise ValueError("eps must be finite and not negative, or None")
     weights = [t for t in (q_weight, k_weight) if t is not None]
     for t in weights:

@@ -7,7 +7,6 @@ accumulation, with no quantisation, clustering or schedule."""
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -41,7 +40,7 @@ def window_attention(q, k, v, *, window=(None, None), sinks=0, causal=False, q_o
     Returns [B, H, Sq, D], or writes ``out``, which shares no memory with an
     input.  The call only queues work on the current stream, and its result
     carries no gradient; ``status`` is as for ``linear``."""
-    if len(window) != 2:
+    if not isinstance(window, (tuple, list)) or len(window) != 2:
         raise ValueError("window must be (left, right)")
     key = ("window", _meta(q), _meta(k), _meta(v), *window, *(type(w) for w in window), sinks, type(sinks), bool(causal),
            q_offset, type(q_offset), _meta(kv_lens), scale, _meta(out), _meta(status))
@@ -87,7 +86,7 @@ def _window_plan(q, k, v, window, sinks, causal, q_offset, kv_lens, scale, out, 
                                 kv_lens.device != q.device):
         raise ValueError("kv_lens must be an int32 tensor [B] on the inputs' device")
     scale = d ** -0.5 if scale is None else scale
-    if not math.isfinite(scale) or not 1e-30 <= scale <= 1e30:
+    if not isinstance(scale, (int, float)) or not 1e-30 <= scale <= 1e30:
         raise ValueError("scale must be positive and finite, in [1e-30, 1e30]")
     _check_status(status, q.device)
     if out is not None:
