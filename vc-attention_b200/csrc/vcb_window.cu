@@ -166,8 +166,9 @@ template <int HD, int NQ> struct WinTile {
     // tensor memory: S (P over it) and O of each query tile
     static constexpr uint32_t kCols = NQ == 2 ? 512 : 256;
     static constexpr uint32_t kColO = NQ * 128;
-    // setmaxnreg shares: control warps, softmax warps
-    static constexpr int kRegsCtl = 64, kRegsSoft = NQ == 2 ? 104 : 88;
+    // setmaxnreg shares: control warps, softmax warps (64 / 104 with two query
+    // tiles: 5.23 ms against 5.15)
+    static constexpr int kRegsCtl = NQ == 2 ? 32 : 64, kRegsSoft = NQ == 2 ? 112 : 88;
     static constexpr int kRegSplit = 128 * kRegsCtl + 256 * NQ * kRegsSoft;
     static_assert(kSmem <= 232448 / kCtas - (kCtas - 1) * 1024, "shared memory of one CTA");
 };
@@ -324,6 +325,9 @@ __device__ __forceinline__ void mma_commit_elected(uint64_t* bar) {
 
 template <typename L>
 __device__ void win_producer(const WinParams& p, const WinItem& it, int fix, uint8_t* smem, const WinBars& B, volatile int* abort) {
+    prefetch_tmap(&p.tm_q);
+    prefetch_tmap(&p.tm_k);
+    prefetch_tmap(&p.tm_v);
     mbar_arrive_expect_tx(B.q_full, it.nq * L::kBytes);
     for (int w = 0; w < it.nq; ++w)
         for (int x = 0; x < L::kBoxes; ++x)
@@ -602,11 +606,6 @@ __global__ void __launch_bounds__(WinTile<HD, NQ>::kThreads, WinTile<HD, NQ>::kC
     volatile int* abort = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;      // warp: uniform
     const WinItem it = win_item<NQ>(p);
-    if (threadIdx.x == 32) {             // while the barriers are set up
-        prefetch_tmap(&p.tm_q);
-        prefetch_tmap(&p.tm_k);
-        prefetch_tmap(&p.tm_v);
-    }
     if (threadIdx.x == 0) {
         mbar_init(B.q_full, 1);
         for (int s = 0; s < L::kStages; ++s) {
