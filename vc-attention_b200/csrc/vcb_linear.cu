@@ -54,10 +54,11 @@ constexpr int kGroup = 12;
 constexpr int kEpiWarps = 8;
 constexpr uint32_t kEpiBytes = 32 * 32 * 4;        // one epilogue warp's staging block
 
+// Shared and tensor memory for tiles of up to BN columns (a launch's are p.bn).
 template <int BN> struct Tile {
     static constexpr uint32_t kBBytes = BN / 2 * kBK * 2;
     static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-    static constexpr int kStages = BN == 256 ? 6 : BN == 128 ? 7 : 8;
+    static constexpr int kStages = BN == 256 ? 6 : 7;
     static constexpr uint32_t kOffEpi = kStages * kStageBytes;
     static constexpr uint32_t kOffBars = kOffEpi + kEpiWarps * kEpiBytes;
     static constexpr int kNumBars = 2 * kStages + 2 + 2 + 1;
@@ -71,6 +72,7 @@ template <int BN> struct Tile {
 struct LinParams {
     CUtensorMap tm_x;            // [batch][head][token][channel]
     CUtensorMap tm_w;            // [n][head][channel]
+    int bn;                      // columns of a tile: a multiple of 32
     int k_chunks, chunks_per_head;
     int m_tiles, n_tiles, m_tiles_per_batch;
     int64_t rows;                // rows of one walk (tokens, or batch x tokens when collapsed)
@@ -79,7 +81,7 @@ struct LinParams {
     int n, n_head;
     int dp_tiles;                // tiles walked whole; the rest is cut along K
     int cut_units, cut_each;     // chunks of the cut tiles, and of one pair's share
-    float* part;                 // [2 per pair][256][BN]
+    float* part;                 // [2 per pair][256][bn]
     int activation;
     const void* bias;
     const void* gate;
@@ -91,24 +93,57 @@ struct LinParams {
     int32_t* status;
 };
 
-__device__ __forceinline__ void tma_load_4d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z,
-                                                 int w) {
+// One stage, by the elected lane of a converged warp (operands in uniform
+// registers, as for the MMAs): expect the pair's bytes (even CTA), load this
+// CTA's x rows and w rows.
+__device__ __forceinline__ void load_stage(uint32_t dst_x, uint32_t dst_w, const CUtensorMap* mx, const CUtensorMap* mw,
+                                           uint32_t own_bar, uint32_t bytes, uint32_t bar, int k, int row, int wrow, int head,
+                                           int batch) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5, %6}], [%2];"
-        ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+        "{\n\t.reg .pred q, e;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "setp.ne.and.u32 e, %5, 0, q;\n\t"
+        "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%4], %5;\n\t"
+        "@q cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%2, {%7, %8, %10, %11}], [%6];\n\t"
+        "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%1], [%3, {%7, %10, %9}], [%6];\n\t}"
+        ::"r"(dst_x), "r"(dst_w), "l"(mx), "l"(mw), "r"(own_bar), "r"(bytes), "r"(bar), "r"(k), "r"(row), "r"(wrow),
+          "r"(head), "r"(batch)
         : "memory");
 }
 
+// The whole warp runs the issue loop and one elected lane issues, so that the
+// operands stay in uniform registers: a lone thread's were moved there before
+// every MMA, and a chunk of four took 570 clocks to issue whatever its width.
 __device__ __forceinline__ void mma2_f16(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
                                          uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
         "mov.b64 da, {%1, %3};\n\t"
         "mov.b64 db, {%2, %3};\n\t"
         "setp.ne.b32 p, %5, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %4, p;\n\t}"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %4, p;\n\t}"
         ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// commits of the elected lane's MMAs (the same lane every time)
+__device__ __forceinline__ void commit_both_elected(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+        ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void commit_local_elected(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(smem_u32(bar))
         : "memory");
 }
 
@@ -160,7 +195,8 @@ template <int BN>
 __device__ void lin_producer(const LinParams& p, uint8_t* smem, const LinBars& B, const Waiter& wait, uint32_t rank,
                              int c, int ncl) {
     using L = Tile<BN>;
-    const uint32_t lead = peer_addr(B.full, 0);
+    const uint32_t lead = __shfl_sync(0xffffffffu, peer_addr(B.full, 0), 0), full0 = smem_u32(B.full), base = smem_u32(smem);
+    const uint32_t bytes = 2 * (kABytes + (uint32_t)p.bn / 2 * kBK * 2);
     uint32_t g = 0;
     bool ok = true;
     LinWork wk;
@@ -169,7 +205,7 @@ __device__ void lin_producer(const LinParams& p, uint8_t* smem, const LinBars& B
         tile_at(p, wk.tile, mt, nt);
         const int b = mt / p.m_tiles_per_batch;
         const int row = (mt - b * p.m_tiles_per_batch) * 256 + (int)rank * 128;
-        const int wrow = nt * BN + (int)rank * (BN / 2);
+        const int wrow = nt * p.bn + (int)rank * (p.bn / 2);
         int head = wk.k0 / p.chunks_per_head, x = (wk.k0 - head * p.chunks_per_head) * kBK;
         for (int k = wk.k0; k < wk.k1; ++k, ++g) {
             const int s = g % L::kStages;
@@ -177,10 +213,9 @@ __device__ void lin_producer(const LinParams& p, uint8_t* smem, const LinBars& B
                 ok = false;
                 break;
             }
-            uint8_t* st = smem + s * L::kStageBytes;
-            if (rank == 0) mbar_arrive_expect_tx(&B.full[s], 2 * L::kStageBytes);
-            tma_load_4d_pair(st, &p.tm_x, lead + 8 * s, x, row, head, b);
-            tma_load_3d_pair(st + kABytes, &p.tm_w, lead + 8 * s, x, head, wrow);
+            const uint32_t st = base + s * L::kStageBytes;
+            load_stage(st, st + kABytes, &p.tm_x, &p.tm_w, full0 + 8 * s, rank == 0 ? bytes : 0u, lead + 8 * s, x, row, wrow,
+                       head, b);
             x += kBK;
             if (x >= p.chunks_per_head * kBK) { x = 0; ++head; }
         }
@@ -200,10 +235,11 @@ __device__ void lin_producer(const LinParams& p, uint8_t* smem, const LinBars& B
 }
 
 template <typename T, int BN>
-__device__ void lin_mma(const LinParams& p, uint8_t* smem, const LinBars& B, const Waiter& wait, uint32_t tmem, int c,
+__device__ void lin_mma(const LinParams& p, uint8_t* smem, const LinBars& B, const Waiter& wait, uint32_t tmem0, int c,
                         int ncl) {
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem0, 0);      // uniform
     using L = Tile<BN>;
-    constexpr uint32_t idesc = idesc_f16<T>(256, BN);
+    const uint32_t idesc = idesc_f16<T>(256, p.bn);
     const uint64_t d64 = smem_desc_k128(smem);
     const uint32_t hi = (uint32_t)(d64 >> 32), lo0 = (uint32_t)d64;
     uint32_t g = 0;
@@ -224,11 +260,11 @@ __device__ void lin_mma(const LinParams& p, uint8_t* smem, const LinBars& B, con
             const uint32_t a = lo0 + s * (L::kStageBytes >> 4), w = a + (kABytes >> 4);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) mma2_f16(d, a + 2 * kk, w + 2 * kk, hi, idesc, k > wk.k0 || kk > 0);
-            commit_both(&B.empty[s]);
+            commit_both_elected(&B.empty[s]);
         }
-        if (ok) commit_both(&B.acc_full[buf]);
+        if (ok) commit_both_elected(&B.acc_full[buf]);
     }
-    commit_local_pair(B.drain);
+    commit_local_elected(B.drain);
     drain_wait(B.drain, 0);
 }
 
@@ -322,14 +358,14 @@ __device__ __forceinline__ RowAt row_at(const LinParams& p, int64_t b, int64_t r
     return {b * p.ys_b + s * p.ys_s, b * p.gs_b + s * p.gs_s, b * p.rs_b + s * p.rs_s, row < p.rows};
 }
 
-// Bias, activation and gate on four rows of a 32 x 32 block, eight columns
+// Bias, activation and gate on ROWS rows of a 32 x 32 block, eight columns
 // n .. n + 7 of each (fewer at the last column when not VEC).
-template <bool VEC>
-__device__ __forceinline__ void finish_rows(const LinParams& p, float (&f)[4][8], int n, const RowAt (&at)[4]) {
+template <bool VEC, int ROWS = 4>
+__device__ __forceinline__ void finish_rows(const LinParams& p, float (&f)[4][8], int n, const RowAt* at) {
     float bias[8];
     if (p.bias) load8_any<VEC>(p.bias, n, p.bias_dtype, p.n - n, bias);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
         float gate[8];
         if (p.gate && at[i].live) load8_any<VEC>(p.gate, at[i].g + n, p.gate_dtype, p.n - n, gate);
         if (p.bias) {
@@ -396,11 +432,11 @@ template <typename T, int BN>
 __device__ void lin_epilogue(const LinParams& p, uint8_t* smem, const LinBars& B, const Waiter& wait, uint32_t tmem,
                              uint32_t rank, int c, int ncl, int ew, int lane) {
     using L = Tile<BN>;
-    constexpr int kHalfCols = BN / 2, kChunks = kHalfCols / 32;
     const int quarter = ew & 3, side = ew >> 2;
     const uint32_t lead_free = peer_addr(B.acc_free, 0);
     float4* stage = reinterpret_cast<float4*>(smem + L::kOffEpi + ew * kEpiBytes);
-    const uint32_t trow = tmem + ((uint32_t)(quarter * 32) << 16) + side * kHalfCols;
+    const uint32_t trow = tmem + ((uint32_t)(quarter * 32) << 16);
+    const int chunks = p.bn / 32;                       // 32-column blocks; this warp takes every second one
     const int r0 = lane >> 2, q8 = (lane & 3) * 8;      // this lane's first row and columns in a block
     LinWork wk;
     for (int li = 0; wk.get(p, c, ncl, li); ++li) {
@@ -412,34 +448,35 @@ __device__ void lin_epilogue(const LinParams& p, uint8_t* smem, const LinBars& B
 #pragma unroll
         for (int i = 0; i < 4; ++i) at[i] = row_at(p, tb, row0 + 8 * i);
         float* part = wk.slot < 0 ? nullptr
-                                  : p.part + ((int64_t)wk.slot * 256 + rank * 128 + quarter * 32 + r0) * BN +
-                                        side * kHalfCols + 4 * (lane & 3);
+                                  : p.part + ((int64_t)wk.slot * 256 + rank * 128 + quarter * 32 + r0) * p.bn +
+                                        4 * (lane & 3);
         const uint32_t buf = li & 1;
         // the residual's runs of the next block, a block ahead (no other block's
         // output touches them, so y may be the residual itself)
         const bool ahead = p.vec && p.residual && !part;
         uint4 next[4];
         auto fetch = [&](int ch) {
-            const int n = nt * BN + side * kHalfCols + ch * 32 + q8;
+            const int n = nt * p.bn + ch * 32 + q8;
             if (ahead && n < p.n) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (at[i].live) next[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.residual) + at[i].r + n);
             }
         };
-        fetch(0);
+        fetch(side);
         if (!wait.parked(&B.acc_full[buf], (li >> 1) & 1)) return;
         tc_fence_after();
+        if (side >= chunks) mbar_arrive_cluster_if(lead_free + 8 * buf, lane == 0);
 #pragma unroll 1
-        for (int ch = 0; ch < kChunks; ++ch) {
+        for (int ch = side; ch < chunks; ch += 2) {
             uint4 res[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) res[i] = next[i];
-            if (ch + 1 < kChunks) fetch(ch + 1);
+            if (ch + 2 < chunks) fetch(ch + 2);
             uint32_t r[32];
             tmem_ld32_at<0>(trow + buf * BN + ch * 32, r);
             tmem_wait_ld();
-            if (ch == kChunks - 1) {
+            if (ch + 2 >= chunks) {
                 tc_fence_before();
                 __syncwarp();
                 mbar_arrive_cluster_if(lead_free + 8 * buf, lane == 0);
@@ -450,13 +487,13 @@ __device__ void lin_epilogue(const LinParams& p, uint8_t* smem, const LinBars& B
                     make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
                                 __uint_as_float(r[4 * j + 3]));
             __syncwarp();
-            const int n0 = nt * BN + side * kHalfCols + ch * 32;
+            const int n0 = nt * p.bn + ch * 32;
             if (part) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int row = r0 + 8 * i;
                     if (!at[i].live) continue;
-                    float4* to = reinterpret_cast<float4*>(part + (int64_t)(8 * i) * BN + ch * 32);
+                    float4* to = reinterpret_cast<float4*>(part + (int64_t)(8 * i) * p.bn + ch * 32);
                     to[0] = stage[row * 8 + ((lane & 3) ^ (row & 7))];             // 64-byte runs of a row
                     to[4] = stage[row * 8 + (((lane & 3) + 4) ^ (row & 7))];
                 }
@@ -529,8 +566,8 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_kernel(const __grid_con
                     bars + 2 * L::kStages + 4};
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
     volatile int* abort = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_rank();
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;      // warp: uniform
+    const uint32_t rank = __shfl_sync(0xffffffffu, cluster_rank(), 0);
     const int c = (int)(blockIdx.x >> 1), ncl = (int)(gridDim.x >> 1);
     if (threadIdx.x == 32) {             // while the barriers are set up
         prefetch_tmap(&p.tm_x);
@@ -559,9 +596,9 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_kernel(const __grid_con
     const uint32_t tmem = *tmem_slot;
     const Waiter wait{abort, peer_addr(const_cast<int*>(abort), rank ^ 1u)};
     if (warp == 0) {
-        if (lane == 0) lin_producer<BN>(p, smem, B, wait, rank, c, ncl);
+        lin_producer<BN>(p, smem, B, wait, rank, c, ncl);
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) lin_mma<T, BN>(p, smem, B, wait, tmem, c, ncl);
+        if (rank == 0) lin_mma<T, BN>(p, smem, B, wait, tmem, c, ncl);
     } else if (warp >= 4) {
         lin_epilogue<T, BN>(p, smem, B, wait, tmem, rank, c, ncl, warp - 4, lane);
     }
@@ -577,14 +614,13 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_kernel(const __grid_con
 
 // A cut tile's pieces, added in the order of their chunks, then the epilogue;
 // one thread per row and eight columns.
-template <typename T, int BN>
+template <typename T>
 __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ LinParams p) {
     pdl_wait();
     pdl_open();
-    constexpr int kGroups = BN / 8, kRowsPer = 256 / kGroups;
-    const int t = blockIdx.x / (256 / kRowsPer);             // cut tile
-    const int row = (blockIdx.x % (256 / kRowsPer)) * kRowsPer + threadIdx.x / kGroups;
-    const int col = threadIdx.x % kGroups * 8;
+    const int groups = p.bn / 8, id = blockIdx.x * 256 + threadIdx.x;
+    const int t = id / (256 * groups), in = id - t * (256 * groups);      // cut tile
+    const int row = in / groups, col = (in - row * groups) * 8;
     const int first = t * p.k_chunks, last = first + p.k_chunks - 1;
     const int c0 = first / p.cut_each, c1 = last / p.cut_each;
     if (c0 == c1) return;                                     // one pair had the whole tile
@@ -592,35 +628,34 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
     tile_at(p, p.dp_tiles + t, mt, nt);
     const int tb = mt / p.m_tiles_per_batch;
     const RowAt at = row_at(p, tb, (int64_t)(mt - tb * p.m_tiles_per_batch) * 256 + row);
-    const int n = nt * BN + col;
+    const int n = nt * p.bn + col;
     if (!at.live || n >= p.n) return;
-    float f[8] = {};
-    for (int c = c0; c <= c1; ++c) {
+    float f[4][8] = {};                                       // one row of finish_rows' four
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {                          // (four pieces' reads in flight)
         const int slot = 2 * c + (first > c * p.cut_each ? 1 : 0);
-        const float4* q = reinterpret_cast<const float4*>(p.part + ((int64_t)slot * 256 + row) * BN + col);
+        const float4* q = reinterpret_cast<const float4*>(p.part + ((int64_t)slot * 256 + row) * p.bn + col);
         const float4 a = q[0], b = q[1];
-        f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
-        f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+        f[0][0] += a.x; f[0][1] += a.y; f[0][2] += a.z; f[0][3] += a.w;
+        f[0][4] += b.x; f[0][5] += b.y; f[0][6] += b.z; f[0][7] += b.w;
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        if (n + e >= p.n) break;
-        const float bias = p.bias ? load1_any(p.bias, n + e, p.bias_dtype) : 0.0f;
-        const float res = p.residual ? F16<T>::to(static_cast<const T*>(p.residual)[at.r + n + e]) : 0.0f;
-        f[e] = finish1<T>(p, f[e], bias, n + e, at, res);
-    }
+    const T* res = static_cast<const T*>(p.residual) + at.r + n;
     T* y = static_cast<T*>(p.y) + at.y;
     if (p.vec) {
+        const uint4 add = p.residual ? *reinterpret_cast<const uint4*>(res) : make_uint4(0, 0, 0, 0);
+        finish_rows<true, 1>(p, f, n, &at);
+        if (p.residual) add_residual<T>(f[0], add);
         const int h = n / p.n_head;
-        *reinterpret_cast<uint4*>(y + h * p.ys_h + (n - h * p.n_head)) =
-            make_uint4(F16<T>::two(f[0], f[1]), F16<T>::two(f[2], f[3]), F16<T>::two(f[4], f[5]), F16<T>::two(f[6], f[7]));
+        *reinterpret_cast<uint4*>(y + h * p.ys_h + (n - h * p.n_head)) = pack8<T>(f[0]);
         return;
     }
+    finish_rows<false, 1>(p, f, n, &at);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         if (n + e >= p.n) break;
         const int h = (n + e) / p.n_head;
-        y[h * p.ys_h + (n + e - h * p.n_head)] = F16<T>::one(f[e]);
+        y[h * p.ys_h + (n + e - h * p.n_head)] =
+            F16<T>::one(p.residual ? __fadd_rn(f[0][e], F16<T>::to(res[e])) : f[0][e]);
     }
 }
 
@@ -768,7 +803,7 @@ int launch_tiles(const LinParams& p, int grid_pairs, cudaStream_t st) {
     VCB_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
     if (p.cut_units) {
         const int tiles = p.cut_units / p.k_chunks;
-        VCB_CUDA(launch_pdl(linear_join_kernel<T, BN>, dim3((unsigned)tiles * (BN / 8)), dim3(256), 0, st, p));
+        VCB_CUDA(launch_pdl(linear_join_kernel<T>, dim3((unsigned)tiles * (p.bn / 8)), dim3(256), 0, st, p));
     }
     return VCB_OK;
 }
@@ -824,23 +859,26 @@ LinPlan plan(const vcb_linear_args* a) {
     q.k_chunks = (int)(q.chunks_per_head * q.heads);
     q.m_tiles = (q.rows + 255) / 256 * q.batches;
     // Tile width, and whether the tiles of the last, partly filled round are
-    // cut along K.  Cost in clocks: a 64-channel chunk takes 650 / 490 / 410 with
-    // 256 / 128 / 64 columns (the loads of x and w bind the narrow ones); a cut
-    // adds the join, its launch and the partial sums' way through L2.
+    // cut along K.  Cost in clocks, fitted to timelines of one pair: a 64-channel
+    // chunk takes the longer of its products (2.2 a column) and its loads (60
+    // bytes a clock); the last epilogue 25 a column; a cut writes its sums (28 a
+    // column) and is joined by a second launch (12000).  Widths that fill the
+    // last round win over cuts but for few rows: 512 x 5120 x 5120 BF16 takes
+    // 36 us cut at 256 columns, 23 at 160.
     const int64_t pairs = sm_count() / 2;
-    const int clocks[3] = {650, 490, 410}, widths[3] = {256, 128, 64};
+    const int64_t tile_rows = q.rows < 128 ? q.rows : 128;
     double best = 0;
-    for (int i = 0; i < 3; ++i) {
-        const int bn = widths[i];
+    for (int bn = 256; bn >= 32; bn -= 32) {
         const int64_t tiles = q.m_tiles * ((a->n + bn - 1) / bn), rem = tiles % pairs;
-        const double chunk = clocks[i], tile = chunk * q.k_chunks + 1500;
-        const double whole = (double)((tiles + pairs - 1) / pairs) * tile;
+        const double mul = 2.2 * bn, ld = (128.0 * (double)tile_rows + 64.0 * bn) / 60;
+        const double chunk = (mul > ld ? mul : ld) + 20, tile = chunk * q.k_chunks;
+        const double whole = (double)((tiles + pairs - 1) / pairs) * tile + 25 * bn;
         int64_t each = (rem * q.k_chunks + pairs - 1) / pairs;
         if (each < 4) each = 4;
-        const double cut = (double)(tiles / pairs) * tile + (double)each * chunk + 1500 + 5000 + (double)rem * bn * 0.4;
+        const double cut = (double)(tiles / pairs) * tile + (double)each * chunk + 28 * bn + 12000;
         const bool use_cut = rem && each < q.k_chunks && cut < whole;
         const double cost = use_cut ? cut : whole;
-        if (i && cost >= best) continue;
+        if (best > 0 && cost >= best) continue;
         best = cost;
         q.bn = bn;
         q.tiles = tiles;
@@ -931,6 +969,7 @@ int linear_run(const vcb_linear_args* a, cudaStream_t st) {
         int rc = make_map16(&p.tm_w, w, bf16, 3, dims, strides, box);
         if (rc) return rc;
     }
+    p.bn = q.bn;
     p.chunks_per_head = q.chunks_per_head;
     p.k_chunks = q.k_chunks;
     p.m_tiles = (int)q.m_tiles;
@@ -942,14 +981,9 @@ int linear_run(const vcb_linear_args* a, cudaStream_t st) {
     p.cut_units = (int)q.cut_units;
     p.cut_each = (int)q.cut_each;
     p.part = reinterpret_cast<float*>(ws + q.off_part);
-    if (bf16) {
-        if (q.bn == 256) return launch_tiles<__nv_bfloat16, 256>(p, q.grid_pairs, st);
-        if (q.bn == 128) return launch_tiles<__nv_bfloat16, 128>(p, q.grid_pairs, st);
-        return launch_tiles<__nv_bfloat16, 64>(p, q.grid_pairs, st);
-    }
-    if (q.bn == 256) return launch_tiles<__half, 256>(p, q.grid_pairs, st);
-    if (q.bn == 128) return launch_tiles<__half, 128>(p, q.grid_pairs, st);
-    return launch_tiles<__half, 64>(p, q.grid_pairs, st);
+    if (q.bn > 128)
+        return bf16 ? launch_tiles<__nv_bfloat16, 256>(p, q.grid_pairs, st) : launch_tiles<__half, 256>(p, q.grid_pairs, st);
+    return bf16 ? launch_tiles<__nv_bfloat16, 128>(p, q.grid_pairs, st) : launch_tiles<__half, 128>(p, q.grid_pairs, st);
 }
 
 }  // namespace vcb
