@@ -860,22 +860,22 @@ LinPlan plan(const vcb_linear_args* a) {
     q.m_tiles = (q.rows + 255) / 256 * q.batches;
     // Tile width, and whether the tiles of the last, partly filled round are
     // cut along K.  Cost in clocks, fitted to timelines of one pair: a 64-channel
-    // chunk takes the longer of its products (2.2 a column) and its loads (60
+    // chunk takes the longer of its products (2.2 a column) and its loads (100
     // bytes a clock); the last epilogue 25 a column; a cut writes its sums (28 a
-    // column) and is joined by a second launch (12000).  Widths that fill the
-    // last round win over cuts but for few rows: 512 x 5120 x 5120 BF16 takes
-    // 36 us cut at 256 columns, 23 at 160.
+    // column) and is joined by a second launch (24000).  A width that fills the
+    // last round is mostly better than a cut: 256 x 5120 x 5120 BF16 takes 24.6 us
+    // cut at 256 columns, 16.7 whole at 96.
     const int64_t pairs = sm_count() / 2;
     const int64_t tile_rows = q.rows < 128 ? q.rows : 128;
     double best = 0;
     for (int bn = 256; bn >= 32; bn -= 32) {
         const int64_t tiles = q.m_tiles * ((a->n + bn - 1) / bn), rem = tiles % pairs;
-        const double mul = 2.2 * bn, ld = (128.0 * (double)tile_rows + 64.0 * bn) / 60;
+        const double mul = 2.2 * bn, ld = (128.0 * (double)tile_rows + 64.0 * bn) / 100;
         const double chunk = (mul > ld ? mul : ld) + 20, tile = chunk * q.k_chunks;
         const double whole = (double)((tiles + pairs - 1) / pairs) * tile + 25 * bn;
         int64_t each = (rem * q.k_chunks + pairs - 1) / pairs;
         if (each < 4) each = 4;
-        const double cut = (double)(tiles / pairs) * tile + (double)each * chunk + 28 * bn + 12000;
+        const double cut = (double)(tiles / pairs) * tile + (double)each * chunk + 28 * bn + 24000;
         const bool use_cut = rem && each < q.k_chunks && cut < whole;
         const double cost = use_cut ? cut : whole;
         if (best > 0 && cost >= best) continue;

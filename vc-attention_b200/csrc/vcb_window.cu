@@ -243,11 +243,22 @@ template <int NQ> __device__ __forceinline__ WinItem win_item(const WinParams& p
     return it;
 }
 
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+// The whole warp runs the load loop and one elected lane issues, as for the MMAs.
+__device__ __forceinline__ void expect_elected(uint32_t bar, uint32_t bytes) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5, %6}], [%2];"
-        ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}"
+        ::"r"(bar), "r"(bytes)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];\n\t}"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
 // D[128 x N] (+)= A B, A and B in shared memory.  The whole warp runs the issue
@@ -328,21 +339,22 @@ __device__ void win_producer(const WinParams& p, const WinItem& it, int fix, uin
     prefetch_tmap(&p.tm_q);
     prefetch_tmap(&p.tm_k);
     prefetch_tmap(&p.tm_v);
-    mbar_arrive_expect_tx(B.q_full, it.nq * L::kBytes);
+    const uint32_t base = smem_u32(smem), q_bar = smem_u32(B.q_full), full0 = smem_u32(B.kv_full), last = smem_u32(B.v_last);
+    const int h = (int)it.h, b = (int)it.b;
+    expect_elected(q_bar, it.nq * L::kBytes);
     for (int w = 0; w < it.nq; ++w)
         for (int x = 0; x < L::kBoxes; ++x)
-            tma_load_4d(smem + w * L::kBytes + x * L::kBox, &p.tm_q, B.q_full, 64 * x, (int)it.row0 + 128 * w, (int)it.h,
-                        (int)it.b);
+            tma_load_4d(base + w * L::kBytes + x * L::kBox, &p.tm_q, q_bar, 64 * x, (int)it.row0 + 128 * w, h, b);
     int issued = 0;
     for (int g = 0; g < 2 * it.count; ++g) {                     // K_0, V_0, K_1, V_1, ...
         const int s = g % L::kStages;
         if (g >= L::kStages && !mbar_wait(&B.kv_empty[s], ((g / L::kStages) - 1) & 1, abort)) break;
         const int key = it.tile(g >> 1) * kKT;
-        uint64_t* bar = g == 2 * fix + 1 ? B.v_last : &B.kv_full[s];
-        mbar_arrive_expect_tx(bar, L::kBytes);
-        uint8_t* st = smem + L::kOffKV + s * L::kBytes;
+        const uint32_t bar = g == 2 * fix + 1 ? last : full0 + 8 * s, st = base + L::kOffKV + s * L::kBytes;
+        expect_elected(bar, L::kBytes);
+#pragma unroll
         for (int x = 0; x < L::kBoxes; ++x)
-            tma_load_4d(st + x * L::kBox, g & 1 ? &p.tm_v : &p.tm_k, bar, 64 * x, key, (int)it.h, (int)it.b);
+            tma_load_4d(st + x * L::kBox, g & 1 ? &p.tm_v : &p.tm_k, bar, 64 * x, key, h, b);
         issued = g + 1;
     }
     if (*abort) {                                                // no copy may land after the CTA exits
@@ -641,7 +653,7 @@ __global__ void __launch_bounds__(WinTile<HD, NQ>::kThreads, WinTile<HD, NQ>::kC
     if (warp < 4) {
         reg_dealloc<L::kRegsCtl>();
         if (it.count > 0) {
-            if (warp == 0 && lane == 0) win_producer<L>(p, it, fix, smem, B, abort);
+            if (warp == 0) win_producer<L>(p, it, fix, smem, B, abort);
             if (warp == 1) win_mma<T, HD, NQ>(it, smem, B, tmem, abort);
             if (warp == 2 && fix >= 0) {
                 const int s = (2 * fix + 1) % L::kStages;
