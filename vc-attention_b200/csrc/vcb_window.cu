@@ -167,8 +167,8 @@ template <int HD, int NQ> struct WinTile {
     static constexpr uint32_t kCols = NQ == 2 ? 512 : 256;
     static constexpr uint32_t kColO = NQ * 128;
     // setmaxnreg shares: control warps, softmax warps (64 / 104 with two query
-    // tiles: 5.23 ms against 5.15)
-    static constexpr int kRegsCtl = NQ == 2 ? 32 : 64, kRegsSoft = NQ == 2 ? 112 : 88;
+    // tiles: 5.23 ms against 5.15; 64 / 88 with one spills)
+    static constexpr int kRegsCtl = 32, kRegsSoft = NQ == 2 ? 112 : 104;
     static constexpr int kRegSplit = 128 * kRegsCtl + 256 * NQ * kRegsSoft;
     static_assert(kSmem <= 232448 / kCtas - (kCtas - 1) * 1024, "shared memory of one CTA");
 };
