@@ -297,3 +297,9 @@ def test_layer_chain_runs_as_one_block():
     x.normal_(generator=g)
     graph.replay()
     assert torch.equal(out, block()[-1])
+
+
+def test_preflight_covers_the_layer_operators():
+    from vc_attention_b200 import b200_backend
+    b200_backend._preflight_layer("cuda:0")
+    assert b200_backend.preflight("cuda:0")["preflight"] == "passed"

@@ -248,8 +248,34 @@ def wait_selftest(complete=False, device="cuda:0"):
             "elapsed_ms": elapsed_ms, "status": status}
 
 
+def _preflight_layer(device):
+    """Known answers of the operators around the attention, on data that 16 bits
+    hold exactly."""
+    from .layer import linear, qk_norm_rope
+    from .window import window_attention
+
+    x = torch.full((1, 37, 96), 2.0, device=device, dtype=torch.bfloat16)
+    w = torch.full((40, 96), 0.25, device=device, dtype=torch.bfloat16)
+    bias = torch.full((40,), 16.0, device=device)
+    for rows in (1, 37):                       # the few-rows kernel and the tensor-core tiles
+        y = linear(x[:, :rows], w, bias, activation="relu", residual=torch.full_like(x[:, :rows, :40], -1.0))
+        torch.testing.assert_close(y, torch.full_like(y, 63.0), rtol=0, atol=0)
+    q = torch.full((1, 1, 19, 16), 3.0, device=device)
+    quarter = torch.ones((19, 8), device=device)
+    turned, _ = qk_norm_rope(q, q, cos=torch.zeros_like(quarter), sin=quarter, eps=0.0)
+    expect = torch.tensor([-1.0, 1.0], device=device).repeat(8).expand_as(turned)
+    torch.testing.assert_close(turned, expect, rtol=1e-6, atol=1e-6)
+    k = torch.zeros((1, 1, 300, 16), device=device, dtype=torch.bfloat16)
+    v = torch.arange(300, device=device, dtype=torch.bfloat16).view(1, 1, 300, 1).expand(1, 1, 300, 16)
+    near = window_attention(k[:, :, :150], k, v, window=(1, 1), q_offset=0)
+    want = torch.arange(150, device=device, dtype=torch.float32).view(1, 1, 150, 1).expand(near.shape).clone()
+    want[:, :, 0] = 0.5                        # the first token sees keys 0 and 1
+    torch.testing.assert_close(near.float(), want, rtol=2.0 ** -7, atol=0)
+
+
 def preflight(device="cuda:0"):
-    """Fail loudly unless ExpCast bytes and the fused FP8 path work (cuda_backend.py:69-88)."""
+    """Fail loudly unless ExpCast bytes and the fused FP8 path work
+    (cuda_backend.py:69-88), and the operators around it."""
     from .core import Config, attention
 
     device = torch.device(device)
@@ -267,6 +293,7 @@ def preflight(device="cuda:0"):
     for cast in (False, True):
         actual, _ = attention(q, k, v, Config(expcast=cast))
         torch.testing.assert_close(actual, torch.full_like(actual, 3), rtol=2e-5, atol=2e-5)
+    _preflight_layer(device)
     torch.cuda.synchronize(device)
     return {"device": str(device), "name": torch.cuda.get_device_name(device), "preflight": "passed",
             **build_info()}

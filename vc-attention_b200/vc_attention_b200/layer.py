@@ -14,8 +14,8 @@ import math
 import torch
 
 from . import _abi
-from .b200_backend import _DTYPES, _extension, _require_b200
 
+_TYPES = {torch.float32: _abi.VCB_F32, torch.float16: _abi.VCB_F16, torch.bfloat16: _abi.VCB_BF16}
 ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4}
 
 
@@ -73,6 +73,12 @@ def _same_view(a, b):
 _PLANS = {}
 
 
+def _require_b200(t, what):
+    from .b200_backend import _require_b200 as check
+
+    check(t, what)
+
+
 def _meta(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
@@ -90,6 +96,8 @@ class _Plan:
     no contiguous last axis (``copy``)."""
 
     def __init__(self, args, entry, copy=(), workspace=None, operands=()):
+        from .b200_backend import _extension
+
         lib = _extension()
         self.lib, self.entry, self.copy, self.operands = lib, getattr(lib, entry), copy, operands
         self.workspace = None if workspace is None else getattr(lib, workspace)
@@ -152,7 +160,7 @@ def _ptr(t):
 def _side_dtype(t, like, what):
     if t.dtype not in (like.dtype, torch.float32) or t.device != like.device:
         raise ValueError(f"{what} must have the inputs' dtype or float32, on their device")
-    return _DTYPES[t.dtype]
+    return _TYPES[t.dtype]
 
 
 def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, heads_in=False, heads_out=None,
@@ -259,7 +267,7 @@ def _linear_plan(x, weight, bias, activation, gate, residual, heads_in, heads_ou
     gs = gate.expand(b, s, n).stride() if gate is not None else (0, 0)
     rs = (0, 0) if residual is None else (residual.stride(0) if residual.ndim == 3 else 0, residual.stride(-2))
     plan = _Plan(_abi.LinearArgs(
-        dtype=_DTYPES[x.dtype], batch=b, tokens=s, n=n, heads_in=hi, k_head=kh, x_stride_b=xs[0], x_stride_h=xs[1],
+        dtype=_TYPES[x.dtype], batch=b, tokens=s, n=n, heads_in=hi, k_head=kh, x_stride_b=xs[0], x_stride_h=xs[1],
         x_stride_s=xs[2], w_stride=weight.stride(0) if n > 1 else k, bias_dtype=bias_dtype,
         activation=ACTIVATIONS[activation], gate_dtype=gate_dtype, gate_stride_b=gs[0], gate_stride_s=gs[1],
         residual_stride_b=rs[0], residual_stride_s=rs[1], n_head=n_head, y_stride_b=ys[0], y_stride_h=ys[1],
@@ -334,7 +342,7 @@ def _rope_plan(q, k, q_weight, k_weight, cos, sin, eps, interleaved, out):
             raise ValueError(f"{name} must be a nonempty [B, H, S, D] tensor")
     if q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
         raise ValueError("q and k must match in batch, tokens and head dimension")
-    if q.dtype != k.dtype or q.device != k.device or q.dtype not in _DTYPES:
+    if q.dtype != k.dtype or q.device != k.device or q.dtype not in _TYPES:
         raise ValueError("q and k must share a device and an FP32/FP16/BF16 dtype")
     b, h, s, d = q.shape
     if d > 128:
@@ -375,8 +383,8 @@ def _rope_plan(q, k, q_weight, k_weight, cos, sin, eps, interleaved, out):
               for t, o in ((q, out and out[0]), (k, out and out[1])))
     triple = ctypes.c_int64 * 3
     return _Plan(_abi.QKNormRopeArgs(
-        dtype=_DTYPES[q.dtype], batch=b, q_heads=h, k_heads=k.shape[1], tokens=s, d=d, q_stride=triple(*q.stride()[:3]),
+        dtype=_TYPES[q.dtype], batch=b, q_heads=h, k_heads=k.shape[1], tokens=s, d=d, q_stride=triple(*q.stride()[:3]),
         k_stride=triple(*k.stride()[:3]), q_out_stride=triple(*qs), k_out_stride=triple(*ks),
-        weight_dtype=_DTYPES[weights[0].dtype] if weights else 0, rows=rows, rotary=rotary, table_stride_b=ts[0],
+        weight_dtype=_TYPES[weights[0].dtype] if weights else 0, rows=rows, rotary=rotary, table_stride_b=ts[0],
         table_stride_s=ts[1], interleaved=int(interleaved), norm=int(eps is not None),
         eps=0.0 if eps is None else float(eps)), "vcb_qk_norm_rope", copy)

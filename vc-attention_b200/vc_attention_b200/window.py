@@ -11,8 +11,8 @@ import ctypes
 import torch
 
 from . import _abi
-from .b200_backend import _DTYPES, _require_b200
-from .layer import _PLANS, _Plan, _check_out, _check_status, _meta, _no_rows, _packed_strides, _ptr, _remember
+from .layer import (_PLANS, _TYPES, _Plan, _check_out, _check_status, _meta, _no_rows, _packed_strides, _ptr, _remember,
+                    _require_b200)
 
 
 def _bound(value, name):
@@ -94,7 +94,7 @@ def _window_plan(q, k, v, window, sinks, causal, q_offset, kv_lens, scale, out, 
     _require_b200(q, "window_attention")
     triple = ctypes.c_int64 * 3
     return _Plan(_abi.WindowArgs(
-        dtype=_DTYPES[q.dtype], batch=b, heads=h, sq=sq, sk=k.shape[2], d=d, q_stride=triple(*q.stride()[:3]),
+        dtype=_TYPES[q.dtype], batch=b, heads=h, sq=sq, sk=k.shape[2], d=d, q_stride=triple(*q.stride()[:3]),
         k_stride=triple(*k.stride()[:3]), v_stride=triple(*v.stride()[:3]),
         out_stride=triple(*(_packed_strides(q.shape) if out is None else out.stride()[:3])), left=left, right=right,
         sinks=first, causal=int(causal), has_offset=int(q_offset is not None), q_offset=q_offset or 0,
