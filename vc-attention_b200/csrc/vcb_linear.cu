@@ -9,8 +9,9 @@
 // rows, the weights' N K bytes below.
 //
 // Work decomposition.  Two CTAs form a cluster; the pair's tile is 256 rows of
-// x by BN rows of w, multiplied by tcgen05.mma.cta_group::2 (M = 256), issued
-// by one thread of the even CTA.  Each CTA loads its 128 rows of x and half of
+// x by bn rows of w (a multiple of 32, up to 256, chosen in plan()), multiplied by
+// tcgen05.mma.cta_group::2 (M = 256), issued by an elected lane of a converged warp
+// of the even CTA: the loop of a lone thread took 570 clocks per 64 channels.  Each CTA loads its 128 rows of x and half of
 // the w rows, 64 channels (128 swizzled bytes) a stage.  K is walked head by
 // head: x is [batch, head, token, channel] and w [n, head, channel] to the
 // TMA (one head for token-major x), and channels behind a head's last are
@@ -31,9 +32,13 @@
 // tile goes to the workspace in FP32, and linear_join_kernel adds a tile's
 // pieces in order and runs the epilogue.
 //
-// Up to 32 rows the product is a stream over w: linear_few_kernel reads w
+// Up to kFewRows rows the product is a stream over w: linear_few_kernel reads w
 // straight into mma.sync fragments (tcgen05 would spend its 128-row tile on
-// them), 16 or 32 rows of w per CTA, K dealt to its eight warps.
+// them), 16 rows of w per CTA, K dealt to its eight warps.
+//
+// Measured, 1 B200, BF16: 32768 x 5120 x 15360 3.77-3.88 ms (1330-1370 TFLOP/s) at
+// the power limit; 8192 x 5120 x 5120 270 us with the tensor pipe 89 % active;
+// 64 rows 16 us; one row 15.5 us cold (52 MB), 10.2 us with w in L2.
 //
 // Operands that TMA cannot address (rows or bases off the 16-byte grid) are
 // first copied, padded, into the caller's workspace.
@@ -49,7 +54,7 @@ constexpr int kLinThreads = 384;
 constexpr int kBK = 64;                            // channels per stage: 128 bytes
 constexpr uint32_t kABytes = 128 * kBK * 2;        // one CTA's x tile of a stage
 // Row tiles that share their walk over w.  32768 x 5120 x 15360 BF16, seconds on end
-// at the power limit: 4 tiles 4.60 ms, 8 4.18, 12 4.12, 16 4.16, 24 4.32, 32 4.57.
+// at the power limit, with an earlier issue loop (now 3.81 ms at 12): 4 tiles 4.60 ms, 8 4.18, 12 4.12, 16 4.16, 24 4.32, 32 4.57.
 constexpr int kGroup = 12;
 constexpr int kEpiWarps = 8;
 constexpr uint32_t kEpiBytes = 32 * 32 * 4;        // one epilogue warp's staging block
@@ -271,8 +276,7 @@ __device__ void lin_mma(const LinParams& p, uint8_t* smem, const LinBars& B, con
 // 0.5 y (1 + erf(y / sqrt 2)) without the cancellation for y < 0: with
 // z = |y| / sqrt 2 and t = 1 / (1 + 0.45 z), erfc(z) = t q(t) exp(-z^2), q a degree-7
 // fit to erfc(z) exp(z^2) / t over z in [0, 60] (least squares reweighted towards
-// the largest relative error, which is 6e-7).  No branches: erfcf's two made this
-// the longest part of a small product (51 us of 771 x 2049 x 1147).
+// the largest relative error, which is 6e-7).  No branches.
 __device__ __forceinline__ float gelu_erf(float y) {
     const float z = 0.70710678118654752f * fabsf(y);
     const float t = __fdividef(1.0f, __fmaf_rn(0.45f, z, 1.0f));
@@ -684,7 +688,7 @@ struct FewParams {
     int k, k_head;
 };
 
-// Few rows (8 NT at most): y^T = w x^T, 16 MT rows of w per CTA.  A lane reads
+// Few rows (8 NT at most): y^T = w x^T, 16 rows of w per CTA.  A lane reads
 // 16-byte runs of w rows (lane / 4) and (lane / 4 + 8), eight channels each, four
 // lanes 64 consecutive bytes, kFewK / 32 runs in flight; x's rows are read with
 // the same assignment of channels to fragment positions (any bijection gives
@@ -693,34 +697,34 @@ struct FewParams {
 // Bound: HBM, w's bytes.
 constexpr int kFewK = 128;
 
-template <typename T, int MT, int NT>
+template <typename T, int NT>
 __global__ void __launch_bounds__(256) linear_few_kernel(const __grid_constant__ FewParams p) {
     pdl_wait();
     pdl_open();
     constexpr int kU = kFewK / 32;
-    __shared__ float part[8][MT * 16][NT * 8 + 1];
+    __shared__ float part[8][16][NT * 8 + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int n0 = blockIdx.x * (16 * MT);
+    const int n0 = blockIdx.x * 16;
     const int rows = (int)p.l.rows;
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    const uint16_t* wrow[2 * MT];
+    const uint16_t* wrow[2];
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) wrow[i] = p.w + (int64_t)(n0 + 8 * i + g) * p.w_stride;
+    for (int i = 0; i < 2; ++i) wrow[i] = p.w + (int64_t)(n0 + 8 * i + g) * p.w_stride;
     const uint16_t* xrow[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         const int r = 8 * j + g, b = r / (int)p.l.tokens;
         xrow[j] = p.x + b * p.xs_b + (r - b * (int)p.l.tokens) * p.xs_s;
     }
-    float acc[MT][NT][4] = {};
+    float acc[NT][4] = {};
     for (int k0 = warp * kFewK; k0 < p.k; k0 += 8 * kFewK) {
-        uint4 wv[kU][2 * MT], xv[kU][NT];
+        uint4 wv[kU][2], xv[kU][NT];
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             const int k = k0 + 32 * u + 8 * t;
             const bool in = k < p.k;
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i)
+            for (int i = 0; i < 2; ++i)
                 wv[u][i] = in && n0 + 8 * i + g < p.l.n ? __ldg(reinterpret_cast<const uint4*>(wrow[i] + k)) : zero;
             const int h = k / p.k_head;
 #pragma unroll
@@ -730,28 +734,24 @@ __global__ void __launch_bounds__(256) linear_few_kernel(const __grid_constant__
                                : zero;
         }
 #pragma unroll
-        for (int u = 0; u < kU; ++u)
+        for (int u = 0; u < kU; ++u) {
+            const uint32_t a0[4] = {wv[u][0].x, wv[u][1].x, wv[u][0].y, wv[u][1].y};
+            const uint32_t a1[4] = {wv[u][0].z, wv[u][1].z, wv[u][0].w, wv[u][1].w};
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const uint32_t a0[4] = {wv[u][2 * i].x, wv[u][2 * i + 1].x, wv[u][2 * i].y, wv[u][2 * i + 1].y};
-                const uint32_t a1[4] = {wv[u][2 * i].z, wv[u][2 * i + 1].z, wv[u][2 * i].w, wv[u][2 * i + 1].w};
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    mma16816<T>(acc[i][j], a0, xv[u][j].x, xv[u][j].y);
-                    mma16816<T>(acc[i][j], a1, xv[u][j].z, xv[u][j].w);
-                }
+            for (int j = 0; j < NT; ++j) {
+                mma16816<T>(acc[j], a0, xv[u][j].x, xv[u][j].y);
+                mma16816<T>(acc[j], a1, xv[u][j].z, xv[u][j].w);
             }
+        }
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) part[warp][16 * i + g + 8 * (e >> 1)][8 * j + 2 * t + (e & 1)] = acc[i][j][e];
+        for (int e = 0; e < 4; ++e) part[warp][g + 8 * (e >> 1)][8 * j + 2 * t + (e & 1)] = acc[j][e];
     __syncthreads();
     // one thread per output element; consecutive threads, consecutive columns of y
-    for (int o = threadIdx.x; o < MT * 16 * NT * 8; o += 256) {
-        const int r = o / (MT * 16), c = o - r * (MT * 16), n = n0 + c;
+    for (int o = threadIdx.x; o < 16 * NT * 8; o += 256) {
+        const int r = o / 16, c = o - r * 16, n = n0 + c;
         if (r >= rows || n >= p.l.n) continue;
         float f = 0.0f;
 #pragma unroll
@@ -765,13 +765,12 @@ __global__ void __launch_bounds__(256) linear_few_kernel(const __grid_constant__
     }
 }
 
-template <typename T, int MT, int NT> int launch_few(const FewParams& p, cudaStream_t st) {
-    VCB_CUDA(launch_pdl(linear_few_kernel<T, MT, NT>, dim3((unsigned)((p.l.n + 16 * MT - 1) / (16 * MT))), dim3(256), 0,
-                        st, p));
+template <typename T, int NT> int launch_few(const FewParams& p, cudaStream_t st) {
+    VCB_CUDA(launch_pdl(linear_few_kernel<T, NT>, dim3((unsigned)((p.l.n + 15) / 16)), dim3(256), 0, st, p));
     return VCB_OK;
 }
 template <typename T> int launch_few_any(const FewParams& p, cudaStream_t st) {
-    return p.l.rows <= 8 ? launch_few<T, 1, 1>(p, st) : launch_few<T, 1, 2>(p, st);
+    return p.l.rows <= 8 ? launch_few<T, 1>(p, st) : launch_few<T, 2>(p, st);
 }
 
 template <typename T, int BN>

@@ -8,7 +8,9 @@
 // normed.  All arithmetic is FP32 and rounds once, at the store.
 //
 // Bound: HBM.  Q and K are read and written once and the tables once (their
-// rows are shared by all heads of a token).
+// rows are shared by all heads of a token).  Measured, 1 B200: 32768 tokens x 40
+// heads x 128, BF16, 237-246 us, 85-89 % of a plain copy's rate; 2 x 24 heads x 4399
+// tokens x 96, FP16, 40 us, bound by issue slots (12 of 16 lanes have channels).
 //
 // Split.  A row of D channels is held by LPR lanes with one 16-byte vector
 // each (16 lanes for 128 16-bit channels), so the sum of squares takes

@@ -30,11 +30,11 @@
 // the time: the kernel runs at the power limit, where every instruction counts.)
 //
 // Measured, 1 B200: 40 heads of 32768 tokens, window 4096 + 4096, 1024 first
-// tokens, BF16: 5.27 ms back to back, 1090 TFLOP/s at the 1000 W limit (the
-// tensor pipe is active 59 % of a 1.6 GHz clock).  Tried without gain: the keys'
+// tokens, BF16: 5.10-5.19 ms back to back, 1108-1126 TFLOP/s at the 1000 W limit
+// and 1.56-1.60 GHz.  Tried without gain: the keys'
 // tiles on CTA pairs with two S and two P buffers (5.72 ms), one thread per row
-// (5.96), part of the exponentials as polynomials (5.37-5.96), no maximum but a
-// check of the sums (5.26, with a second path).
+// (5.96), no maximum but a check of the sums (5.26, no gain
+// for a second path), part of the exponentials as polynomials (5.15-5.17 against 5.19).
 //
 // A masked key has P = 0, but 0 times a NaN or infinity in its V row would
 // still reach O.  Rows behind a batch entry's last key are therefore cleared in
