@@ -378,3 +378,17 @@ def test_calls_of_one_shape_from_two_threads():
     for t in threads:
         t.join()
     assert not bad
+
+
+def test_rope_one_token_with_tables_from_two_caches():
+    from vc_attention_b200 import qk_norm_rope
+    g = _gen(77)
+    q, k = _randn((2, 3, 1, 64), BF16, g), _randn((2, 1, 1, 64), BF16, g)
+    cos_cache = _tables(9, 32, g)[0]
+    for start in (0, 4, 5):                     # the second table on and off the 16-byte grid
+        sin_cache = _tables(9, 48, g)[1][:, start:start + 32]
+        cos, sin = cos_cache[5:6], sin_cache[5:6]
+        for c, s in ((cos, sin), (sin, cos), (cos[None], sin[None])):
+            qo, ko = qk_norm_rope(q, k, None, None, c, s)
+            _check(qo, *_rope_ref(q, None, c, s, True, 1e-6))
+            _check(ko, *_rope_ref(k, None, c, s, True, 1e-6))

@@ -4,7 +4,7 @@ import ctypes
 import pytest
 import torch
 
-from vc_attention_b200 import _abi, linear, qk_norm_rope, window_attention
+from vc_attention_b200 import _abi, layer, linear, qk_norm_rope, window_attention
 from vc_attention_b200.layer import _overlaps_itself, _shares_memory
 
 BF16 = torch.bfloat16
@@ -185,3 +185,29 @@ def test_window_c_entry_refuses_without_a_device():
         assert lib.vcb_window_attention(ctypes.byref(a), None) == _abi.VCB_ERR_INVALID_ARGUMENT
         assert match in _abi.last_error(lib)
         setattr(a, field, keep)
+
+
+def test_tables_of_one_row_from_two_caches_are_not_copied_forever(monkeypatch):
+    """One token's rows of tables with different row strides: contiguous()
+    returns them unchanged, so they must not count as different."""
+    calls = []
+
+    class Plan:
+        def __init__(self, args, entry, copy=(), *rest):
+            self.copy = copy
+
+        def call(self, device, **pointers):
+            calls.append(self.copy)
+
+    monkeypatch.setattr(layer, "_require_b200", lambda t, what: None)
+    monkeypatch.setattr(layer, "_Plan", Plan)
+    monkeypatch.setattr(layer, "_PLANS", {})
+    q = torch.randn(1, 2, 1, 16)
+    cos, sin = torch.randn(5, 8)[2:3], torch.randn(5, 16)[2:3, :8]
+    assert cos.stride() != sin.stride()
+    layer.qk_norm_rope(q, q, cos=cos, sin=sin)
+    layer.qk_norm_rope(q, q, cos=cos[None], sin=sin[None].expand(1, 1, 8))
+    assert calls == [(), ()]
+    q = torch.randn(1, 2, 5, 16)
+    layer.qk_norm_rope(q, q, cos=torch.randn(5, 8), sin=torch.randn(5, 16)[:, :8])     # these do differ: copied once
+    assert calls == [(), (), ()]

@@ -132,6 +132,12 @@ def _no_rows(t):
     return t is not None and t.shape[-1] != 1 and t.stride(-1) != 1
 
 
+def _strides_differ(a, b):
+    """Whether two tensors of one shape step differently.  Axes of length one
+    do not step: contiguous() leaves their strides as they are."""
+    return any(n > 1 and i != j for n, i, j in zip(a.shape, a.stride(), b.stride()))
+
+
 def _check_out(out, shape, like, what, inputs, may_be=None):
     """An output the caller gives: shape, type, device, a contiguous last axis,
     no overlap with itself or with an input other than ``may_be`` itself."""
@@ -309,7 +315,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, *, eps=
     if out is not None:
         _check_rope_out(out, q, k, q_weight, k_weight, cos, sin)
     if plan.copy:
-        if cos is not None and cos.stride() != sin.stride():
+        if cos is not None and _strides_differ(cos, sin):
             cos, sin = cos.contiguous(), sin.contiguous()
         q, k, q_weight, k_weight, cos, sin = (t.contiguous() if _no_rows(t) else t
                                               for t in (q, k, q_weight, k_weight, cos, sin))
@@ -373,7 +379,7 @@ def _rope_plan(q, k, q_weight, k_weight, cos, sin, eps, interleaved, out):
             raise ValueError("the tables rotate more channels than a head has")
         if cos.ndim == 3 and cos.shape[0] not in (1, b):
             raise ValueError("batched tables need one entry, or one for each batch entry")
-        if cos.stride() != sin.stride():
+        if _strides_differ(cos, sin):
             copy = (*copy, 4, 5)
         ts = (cos.stride(0) if cos.ndim == 3 and cos.shape[0] > 1 else 0, cos.stride(-2))
     if out is not None:
