@@ -11,8 +11,8 @@
 // Work decomposition.  Two CTAs form a cluster; the pair's tile is 256 rows of
 // x by bn rows of w (a multiple of 32, up to 256, chosen in plan()), multiplied by
 // tcgen05.mma.cta_group::2 (M = 256), issued by an elected lane of a converged warp
-// of the even CTA: the loop of a lone thread took 570 clocks per 64 channels.  Each CTA loads its 128 rows of x and half of
-// the w rows, 64 channels (128 swizzled bytes) a stage.  K is walked head by
+// of the even CTA: the loop of a lone thread took 570 clocks per 64 channels.
+// Each CTA loads its 128 rows of x and half of the w rows, 64 channels (128 swizzled bytes) a stage.  K is walked head by
 // head: x is [batch, head, token, channel] and w [n, head, channel] to the
 // TMA (one head for token-major x), and channels behind a head's last are
 // zero-filled on both sides.  The grid is persistent; tiles are walked in
@@ -36,9 +36,10 @@
 // straight into mma.sync fragments (tcgen05 would spend its 128-row tile on
 // them), 16 rows of w per CTA, K dealt to its eight warps.
 //
-// Measured, 1 B200, BF16: 32768 x 5120 x 15360 3.77-3.88 ms (1330-1370 TFLOP/s) at
-// the power limit; 8192 x 5120 x 5120 270 us with the tensor pipe 89 % active;
-// 64 rows 16 us; one row 15.5 us cold (52 MB), 10.2 us with w in L2.
+// Measured, 1 B200, BF16: 32768 x 5120 x 15360 3.72-3.92 ms (1315-1384 TFLOP/s) at
+// the power limit; 8192 x 5120 x 5120 273 us with the tensor pipe 90 % active;
+// 64 rows 15.6 us; one row 15.6 us cold (52 MB), 10.2 us with w in L2; 771 x 1147 x
+// 2049 with GELU and residual, off the 16-byte grid, 25.5 us after a copy of 8 us.
 //
 // Operands that TMA cannot address (rows or bases off the 16-byte grid) are
 // first copied, padded, into the caller's workspace.
@@ -54,7 +55,8 @@ constexpr int kLinThreads = 384;
 constexpr int kBK = 64;                            // channels per stage: 128 bytes
 constexpr uint32_t kABytes = 128 * kBK * 2;        // one CTA's x tile of a stage
 // Row tiles that share their walk over w.  32768 x 5120 x 15360 BF16, seconds on end
-// at the power limit, with an earlier issue loop (now 3.81 ms at 12): 4 tiles 4.60 ms, 8 4.18, 12 4.12, 16 4.16, 24 4.32, 32 4.57.
+// at the power limit, with an earlier issue loop (now 3.72-3.92 ms at 12): 4 tiles
+// 4.60 ms, 8 4.18, 12 4.12, 16 4.16, 24 4.32, 32 4.57.
 constexpr int kGroup = 12;
 constexpr int kEpiWarps = 8;
 constexpr uint32_t kEpiBytes = 32 * 32 * 4;        // one epilogue warp's staging block
@@ -879,7 +881,7 @@ LinPlan plan(const vcb_linear_args* a) {
     // bytes a clock); the last epilogue 25 a column; a cut writes its sums (28 a
     // column) and is joined by a second launch (24000).  A width that fills the
     // last round is mostly better than a cut: 256 x 5120 x 5120 BF16 takes 24.6 us
-    // cut at 256 columns, 16.7 whole at 96.
+    // cut at 256 columns, 16.0 whole at 96.
     const int64_t pairs = sm_count() / 2;
     const int64_t tile_rows = q.rows < 128 ? q.rows : 128;
     double best = 0;
