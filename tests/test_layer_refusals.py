@@ -211,3 +211,52 @@ def test_tables_of_one_row_from_two_caches_are_not_copied_forever(monkeypatch):
     q = torch.randn(1, 2, 5, 16)
     layer.qk_norm_rope(q, q, cos=torch.randn(5, 8), sin=torch.randn(5, 16)[:, :8])     # these do differ: copied once
     assert calls == [(), (), ()]
+
+
+class _NoKernel:
+    """Stands in for a call's plan: no library, no device."""
+
+    def __init__(self, args, entry, copy=(), *rest):
+        self.args, self.entry, self.copy = args, entry, copy
+
+    def call(self, device, **pointers):
+        pass
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """Calls run through their checks and stop before the library."""
+    from vc_attention_b200 import window
+    for module in (layer, window):
+        monkeypatch.setattr(module, "_require_b200", lambda t, what: None)
+        monkeypatch.setattr(module, "_Plan", _NoKernel)
+    monkeypatch.setattr(layer, "_PLANS", plans := {})
+    monkeypatch.setattr(window, "_PLANS", plans)
+
+
+def test_an_output_may_be_one_argument_only(on_cpu):
+    """The tensor that an output may overwrite (the residual; Q for q_out, K for
+    k_out) is not exempt where it is another argument too: the products still
+    read it while the output is written."""
+    x, w = _t(2, 3, 8), _t(8, 8)
+    for _ in range(2):                          # the second time the shapes are known
+        assert linear(x, w, residual=x).shape == x.shape
+        held = _t(2, 3, 8)
+        assert linear(x, w, residual=held, out=held) is held
+        for kw in (dict(residual=x, out=x), dict(residual=held, gate=held, out=held)):
+            with pytest.raises(ValueError, match="share memory"):
+                linear(x, w, **kw)
+    square = _t(8, 8)
+    for _ in range(2):
+        with pytest.raises(ValueError, match="share memory"):
+            linear(_t(8, 8), square, residual=square, out=square)
+    q, k, other = _t(2, 4, 6, 16), _t(2, 4, 6, 16), _t(2, 4, 6, 16)
+    for _ in range(2):
+        assert qk_norm_rope(q, k, out=(q, k)) == (q, k)
+        assert qk_norm_rope(q, q, out=(k, other)) == (k, other)
+        for out in ((q, other), (other, q)):
+            with pytest.raises(ValueError, match="share memory"):
+                qk_norm_rope(q, q, out=out)
+    row = _t(1, 1, 1, 16)
+    with pytest.raises(ValueError, match="share memory"):
+        qk_norm_rope(row, _t(1, 1, 1, 16), row[0, 0, 0], out=(row, _t(1, 1, 1, 16)))

@@ -140,17 +140,19 @@ def _strides_differ(a, b):
 
 def _check_out(out, shape, like, what, inputs, may_be=None):
     """An output the caller gives: shape, type, device, a contiguous last axis,
-    no overlap with itself or with an input other than ``may_be`` itself."""
+    no overlap with itself, with ``inputs``, or with a part of ``may_be``: the
+    argument that it may be itself.  (By argument and not by object: a tensor
+    that is the residual and x too may not be overwritten while x is read.)"""
     if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{what} must be a {tuple(shape)} tensor of the inputs' dtype and device")
     if out.shape[-1] != 1 and out.stride(-1) != 1:
         raise ValueError(f"{what} must have a contiguous last axis")
     if _overlaps_itself(out):
         raise ValueError(f"{what} must not overlap itself")
+    if may_be is not None and not _same_view(out, may_be):
+        inputs = (*inputs, may_be)
     for t in inputs:
-        if t is None or (may_be is not None and t is may_be and _same_view(out, t)):
-            continue
-        if _shares_memory(out, t):
+        if t is not None and _shares_memory(out, t):
             raise ValueError(f"{what} must not share memory with an input")
 
 
@@ -197,7 +199,7 @@ def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, h
         plan = _linear_plan(x, weight, bias, activation, gate, residual, bool(heads_in), heads_out, out, status)
         _remember(key, plan)
     if out is not None:
-        _check_out(out, plan.shape, x, "out", (x, weight, bias, gate, residual), may_be=residual)
+        _check_out(out, plan.shape, x, "out", (x, weight, bias, gate), may_be=residual)
     if plan.copy:
         x, weight, bias, gate, residual = (t.contiguous() if _no_rows(t) else t
                                            for t in (x, weight, bias, gate, residual))
@@ -256,7 +258,7 @@ def _linear_plan(x, weight, bias, activation, gate, residual, heads_in, heads_ou
         raise ValueError("residual must have the result's shape, dtype and device")
     _check_status(status, x.device)
     if out is not None:
-        _check_out(out, shape, x, "out", (x, weight, bias, gate, residual), may_be=residual)
+        _check_out(out, shape, x, "out", (x, weight, bias, gate), may_be=residual)
     _require_b200(x, "linear")
     copy = tuple(i for i, t in enumerate((x, weight, bias, gate, residual)) if _no_rows(t))
     if heads_in:
@@ -298,8 +300,8 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, *, eps=
     are not rotated.  Arithmetic is FP32 with one rounding at the end.
 
     Returns (q, k) as contiguous BNSD tensors, or writes ``out=(q_out,
-    k_out)``, for example rows of a K buffer; an output may be its own
-    input.  The call only queues work on the current stream, and its results
+    k_out)``, for example rows of a K buffer; q_out may be ``q`` itself and
+    k_out ``k``, and neither shares memory with another argument.  The call only queues work on the current stream, and its results
     carry no gradient."""
     if out is None:
         outs = None
@@ -331,8 +333,8 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, *, eps=
 
 
 def _check_rope_out(out, q, k, *others):
-    _check_out(out[0], q.shape, q, "q_out", (q, k, *others), may_be=q)
-    _check_out(out[1], k.shape, k, "k_out", (k, q, *others), may_be=k)
+    _check_out(out[0], q.shape, q, "q_out", (k, *others), may_be=q)
+    _check_out(out[1], k.shape, k, "k_out", (q, *others), may_be=k)
     if _shares_memory(out[0], out[1]):
         raise ValueError("q_out and k_out must not share memory")
 
