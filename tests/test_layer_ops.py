@@ -392,3 +392,16 @@ def test_rope_one_token_with_tables_from_two_caches():
             qo, ko = qk_norm_rope(q, k, None, None, c, s)
             _check(qo, *_rope_ref(q, None, c, s, True, 1e-6))
             _check(ko, *_rope_ref(k, None, c, s, True, 1e-6))
+
+
+def test_linear_few_rows_with_the_longest_sum():
+    """K at the bound that the entry point takes: the walk over K ends there."""
+    from vc_attention_b200 import linear
+    k = 2 ** 31 - 264
+    x = torch.zeros((1, k), device="cuda", dtype=BF16)
+    w = torch.ones((1, k), device="cuda", dtype=BF16)
+    for at, value in ((0, 1.0), (1023, 2.0), (1024, 4.0), (k // 2, 8.0), (k - 1025, 16.0), (k - 1, 32.0)):
+        x[0, at] = value
+    assert linear(x, w).item() == 63.0
+    w[0, k - 1] = 0.5
+    assert linear(x, w).item() == 47.0

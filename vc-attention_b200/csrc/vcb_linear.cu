@@ -731,16 +731,17 @@ __global__ void __launch_bounds__(256) linear_few_kernel(const __grid_constant__
         xrow[j] = p.x + b * p.xs_b + (r - b * (int)p.l.tokens) * p.xs_s;
     }
     float acc[NT][4] = {};
-    for (int k0 = warp * kFewK; k0 < p.k; k0 += 8 * kFewK) {
+    // unsigned: k is below 2^31, and the step past its end must not wrap
+    for (uint32_t k0 = warp * kFewK; k0 < (uint32_t)p.k; k0 += 8 * kFewK) {
         uint4 wv[kU][2], xv[kU][NT];
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            const int k = k0 + 32 * u + 8 * t;
-            const bool in = k < p.k;
+            const uint32_t k = k0 + 32 * u + 8 * t;
+            const bool in = k < (uint32_t)p.k;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 wv[u][i] = in && n0 + 8 * i + g < p.l.n ? __ldg(reinterpret_cast<const uint4*>(wrow[i] + k)) : zero;
-            const int h = k / p.k_head;
+            const uint32_t h = k / (uint32_t)p.k_head;
 #pragma unroll
             for (int j = 0; j < NT; ++j)
                 xv[u][j] = in && 8 * j + g < rows
