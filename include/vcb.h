@@ -306,7 +306,8 @@ VCB_API int vcb_qk_norm_rope(const vcb_qk_norm_rope_args* args, void* stream);
  * p = i + offset (q_offset, or without has_offset the entry's keys - sq, which
  * puts the last query on the last key) and sees key j < keys of its batch entry
  * when (j < sinks or p - left <= j <= p + right) and (not causal or j <= p).
- * out = softmax(scale q . k) v over the seen keys; a row that sees none is 0.
+ * out = softmax(scale q . k) v over the seen keys; a row that sees none is 0,
+ * one whose seen logits are all -inf is NaN (0 / 0).
  * Keys that no row sees do not reach the output, whatever they hold. */
 typedef struct {
     const void* q; const void* k; const void* v;

@@ -303,3 +303,27 @@ def test_preflight_covers_the_layer_operators():
     from vc_attention_b200 import b200_backend
     b200_backend._preflight_layer("cuda:0")
     assert b200_backend.preflight("cuda:0")["preflight"] == "passed"
+
+
+@pytest.mark.parametrize("d", [128, 41])
+@pytest.mark.parametrize("sq,sk", [(1, 40), (1, 3000), (70, 600), (200, 600)])
+def test_window_rows_whose_logits_are_all_minus_infinity(sq, sk, d):
+    """Softmax has no value there (0 / 0) and the output is NaN; zeros are for
+    rows that see no key.  One finite key among them takes the whole weight."""
+    g = _gen(sq + d)
+    q = _randn((2, 2, sq, d), BF16, g).abs() + 0.5
+    k, v = _randn((2, 2, sk, d), BF16, g), _randn((2, 2, sk, d), BF16, g)
+    k[0, 1, :, 0] = -float("inf")
+    lens = [sk, 0]
+    for kw in (dict(), dict(window=(3, 0), causal=True)):
+        got, (ref, err), seen = _run(q, k, v, lens=lens, **kw)
+        _check(got[:1, :1], ref[:1, :1], err[:1, :1])
+        assert got[0, 1].isnan().all()
+        assert (got[1] == 0).all()
+        held = k[0, 1, sk - 2].clone()
+        k[0, 1, sk - 2, 0] = 1.0
+        got, _, _ = _run(q, k, v, lens=lens, **kw)
+        k[0, 1, sk - 2] = held
+        sees = seen[0, :, sk - 2]
+        assert sees.any() and torch.equal(got[0, 1][sees], v[0, 1, sk - 2].expand(int(sees.sum()), d))
+        assert got[0, 1][~sees].isnan().all()

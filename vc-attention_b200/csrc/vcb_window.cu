@@ -96,7 +96,8 @@ __device__ __forceinline__ int64_t keys_of(const WinParams& p, int64_t b) {
 }
 
 // One output row by one warp, reading only the keys that the row sees: lane l
-// takes every 32nd key's logit, then channels l, l + 32, ... of the sum.
+// takes every 32nd key's logit, then channels l, l + 32, ... of the sum.  0 for
+// a row that sees no key; a row whose logits are all -inf is 0 / 0, a NaN.
 // `qrow` is 128 floats of shared memory of this warp.
 template <typename T>
 __device__ void window_row(const WinParams& p, int64_t b, int64_t h, int64_t i, float* qrow, int lane) {
@@ -143,10 +144,11 @@ __device__ void window_row(const WinParams& p, int64_t b, int64_t h, int64_t i, 
             m = m_new;
         }
     }
+    const bool sees = s.sink > 0 || s.hi > s.lo;
     T* out = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + i * p.os[2];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (lane + 32 * e < p.d) out[lane + 32 * e] = F16<T>::one(den == 0.0f ? 0.0f : acc[e] / den);
+        if (lane + 32 * e < p.d) out[lane + 32 * e] = F16<T>::one(sees ? acc[e] / den : 0.0f);
 }
 
 constexpr int kKT = 128;                           // keys per tile
