@@ -327,3 +327,54 @@ def test_window_rows_whose_logits_are_all_minus_infinity(sq, sk, d):
         sees = seen[0, :, sk - 2]
         assert sees.any() and torch.equal(got[0, 1][sees], v[0, 1, sk - 2].expand(int(sees.sum()), d))
         assert got[0, 1][~sees].isnan().all()
+
+
+@pytest.mark.parametrize("sq,sk,d", [(1, 60000, 128), (200, 60000, 128), (300, 60000, 64), (40, 700, 80)])
+def test_window_small_fp16_weights_keep_their_share(sq, sk, d):
+    """One key of value 0 above very many of value 1 with weights near 2^-26
+    each: their sum is the output.  A weight is held as 2^7 w or more, so a step
+    of FP16's smallest numbers is 2^-24 / 2^7, a rounding at most half of it."""
+    q = torch.zeros((1, 2, sq, d), device="cuda", dtype=FP16)
+    k, v = (torch.zeros((1, 2, sk, d), device="cuda", dtype=FP16) for _ in range(2))
+    q[..., 0] = 1.0
+    for first in (0, sk // 2, sk - 1):
+        k[..., 0], v[:] = -18.203125, 1.0
+        k[:, :, first], v[:, :, first] = 0.0, 0.0
+        got, _, _ = _run(q, k, v, q_offset=0, scale=1.0)
+        rest = (sk - 1) * torch.tensor(-18.203125, dtype=torch.float64).exp().item()
+        want = rest / (1 + rest)
+        # the weights' roundings, the exponential's (2^-20 (1 + 18.2) of each), the sums' steps, the store
+        tol = (sk - 1) * 2.0 ** -32 + (2.0 ** -15 + (sk / 16 + 8) * 2.0 ** -22) * want + 2.0 ** -11 * want + 2.0 ** -25
+        assert (got.double() - want).abs().max() <= tol
+
+
+def _tight(q, k, v, seen, scale):
+    """(output, bound) with one rounding of the weights: they are summed before
+    it, so only the product with V takes their half steps, (eps / 2) A, and in
+    FP16 half a step of its smallest numbers, 2^-25 of 2^7 or more: n 2^-32 max |v|.
+    The other terms are those of _reference."""
+    qd, kd, vd = q.double(), k.double(), v.double()
+    hidden = ~seen[:, None]
+    s = (qd @ kd.transpose(-1, -2) * scale).masked_fill(hidden, float("-inf"))
+    mag = (qd.abs() @ kd.abs().transpose(-1, -2) * scale).masked_fill(hidden, 0)
+    w = torch.softmax(s.masked_fill(hidden.all(-1, keepdim=True), 0.0), -1).masked_fill(hidden, 0.0)
+    big = w @ vd.abs()
+    dot = (q.shape[-1] / 16 + 2) * 2.0 ** -22 * mag.amax(-1, keepdim=True)
+    top = s.masked_fill(hidden, 0).abs().amax(-1, keepdim=True)
+    n = seen.sum(-1)[:, None, :, None].double()
+    eps = torch.finfo(q.dtype).eps
+    err = (eps / 2 + 2 * dot + 2.0 ** -20 * (1 + top) + (n / 16 + 8) * 2.0 ** -22) * big
+    if q.dtype == FP16:
+        err = err + n * 2.0 ** -32 * vd.abs().amax(2, keepdim=True)
+    return w @ vd, err
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("mask", range(len(MASKS)))
+@pytest.mark.parametrize("shape", [(1, 2, 1, 700, 128), (1, 2, 130, 260, 96), (2, 1, 515, 515, 41), (1, 1, 300, 5000, 64)])
+def test_window_weights_are_rounded_once(shape, mask, dtype):
+    b, h, sq, sk, d = shape
+    g = _gen(sq + sk + d + mask)
+    q, k, v = (_randn((b, h, n, d), dtype, g, a) for n, a in ((sq, 3.0), (sk, 1.0), (sk, 1.0)))
+    got, _, seen = _run(q, k, v, **MASKS[mask])
+    _check(got, *_tight(q, k, v, seen, d ** -0.5))

@@ -21,13 +21,21 @@
 // softmax; the issue order PV_0(j), QK_0(j+1), PV_1(j), QK_1(j+1) makes S_w(j+1)
 // follow P_w(j) in the same columns without a further wait.
 //
-// The running maximum moves only when a row's maximum passes it by 2^8: until
-// then P just grows, exactly representable in FP32 sums and both 16-bit types,
-// and O is not rescaled.  A softmax warp rescales O itself, between the commit
-// that follows PV_w(j-1) and its own arrival for PV_w(j).  The row sum adds P in
-// FP32, before its rounding: an output is off by the roundings of P, at most half
-// a step each.  (Summing the rounded P costs one instruction per score and 5 % of
-// the time: the kernel runs at the power limit, where every instruction counts.)
+// P = 2^(s - m).  The reference m moves only when a row's maximum passes it by
+// more than 2^8: until then P just grows, and O is not rescaled.  A softmax warp
+// rescales O itself, between the commit that follows PV_w(j-1) and its own
+// arrival for PV_w(j).
+//
+// P has fewer bits than S: it is the A operand of a 16-bit product.  The row sum
+// adds it in FP32, before its rounding, so an output is off by the roundings of P:
+// half a step each, (eps / 2) sum_j w_j |v_j|.  (Summing the rounded P costs one
+// instruction per score and 5 % of the time: the kernel runs at the power limit,
+// where every instruction counts.)  BF16 has FP32's exponents.  FP16 ends at 2^-24,
+// so there m lies 2^7 below the maximum and P reaches 2^15 (the largest FP16 is
+// 65504): weights below 2^-21 of the maximum are off by up to 2^-32 of it, and
+// only those below 2^-32 are lost to the product (2^-25 with m at the maximum,
+// where 60000 keys at 2^-26 lost their whole share).  The sums carry the same
+// factor, so it cancels.
 //
 // Measured, 1 B200: 40 heads of 32768 tokens, window 4096 + 4096, 1024 first
 // tokens, BF16: 5.10-5.19 ms back to back, 1108-1126 TFLOP/s at the 1000 W limit
@@ -456,6 +464,7 @@ __device__ void win_softmax(const WinParams& p, const WinItem& it, uint8_t* smem
     const uint32_t trow = tmem + ((uint32_t)(quarter * 32 + sub * 16) << 16);
     const uint32_t ts = trow + 128 * w, to = trow + L::kColO + 128 * w;
     const float c = p.c;
+    constexpr float kUp = F16<T>::kDtype == VCB_F16 ? 7.0f : 0.0f;      // log2 of P at the row's maximum
     float m = -INFINITY, den = 0.0f;
     for (int j = 0; j < it.count; ++j) {
         if (!mbar_wait(&B.s_full[w], j & 1, abort)) return;
@@ -492,7 +501,7 @@ __device__ void win_softmax(const WinParams& p, const WinItem& it, uint8_t* smem
                 mx[e] = fmax3(mx[e], __uint_as_float(r[8 * t + 2 * e]), __uint_as_float(r[8 * t + 2 * e + 1]));
         float top = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
         top = __fmul_rn(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)), c);
-        const float m_new = top > m + 8.0f ? top : m;
+        const float m_new = top > m + (8.0f + kUp) ? top - kUp : m;
         const float alpha = m_new == m ? 1.0f : ex2_ftz(m - m_new);
         const bool moved = __any_sync(0xffffffffu, m_new != m);
         const float ref = m_new == -INFINITY ? 0.0f : m_new;
