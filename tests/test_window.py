@@ -378,3 +378,22 @@ def test_window_weights_are_rounded_once(shape, mask, dtype):
     q, k, v = (_randn((b, h, n, d), dtype, g, a) for n, a in ((sq, 3.0), (sk, 1.0), (sk, 1.0)))
     got, _, seen = _run(q, k, v, **MASKS[mask])
     _check(got, *_tight(q, k, v, seen, d ** -0.5))
+
+
+@pytest.mark.parametrize("sq,sk,d", [(1, 40, 128), (1, 3000, 128), (70, 600, 80), (200, 600, 41), (300, 300, 64)])
+def test_window_sums_of_the_largest_values_stay_finite(sq, sk, d):
+    """Finite BF16 values whose unnormalised sum passes FP32's range: the mean
+    is in range and must come out."""
+    g = _gen(sq + sk)
+    q, k = _randn((1, 2, sq, d), BF16, g), _randn((1, 2, sk, d), BF16, g)
+    most = torch.finfo(BF16).max
+    v = (torch.rand((1, 2, sk, d), device="cuda", generator=g) * 2 - 1).mul(most).to(BF16)
+    v[:, 1] = most                             # equal values: their mean is the value itself
+    for kw in (dict(), dict(window=(90, 0), causal=True, sinks=7)):
+        got, _, seen = _run(q, k, v, **kw)
+        ref, err = _reference(q.double(), k.double(), v.double(), seen, d ** -0.5)
+        eps = torch.finfo(BF16).eps
+        err = err + (eps + torch.finfo(torch.float32).eps) * most      # (_reference took eps from 64-bit copies)
+        assert got.isfinite().all()
+        assert ((got.double() - ref).abs() <= err + eps / 2 * (ref.abs() + err)).all()
+        assert (got[:, 1][seen.any(-1)] == most).all()

@@ -47,7 +47,8 @@
 // A masked key has P = 0, but 0 times a NaN or infinity in its V row would
 // still reach O.  Rows behind a batch entry's last key are therefore cleared in
 // shared memory, and a row whose sums are not finite is computed again by
-// window_row, which reads only the keys that the row sees.
+// window_row, which reads only the keys that the row sees.  Finite values near
+// the end of BF16's range take that way too: P V sums them before the division.
 //
 // Roles (128 + 128 NQ threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2
 // clears V rows behind the last key, warp 3 tensor memory; then one softmax
@@ -104,8 +105,9 @@ __device__ __forceinline__ int64_t keys_of(const WinParams& p, int64_t b) {
 }
 
 // One output row by one warp, reading only the keys that the row sees: lane l
-// takes every 32nd key's logit, then channels l, l + 32, ... of the sum.  0 for
-// a row that sees no key; a row whose logits are all -inf is 0 / 0, a NaN.
+// takes every 32nd key's logit, then channels l, l + 32, ... of the mean of V so
+// far: a mean of finite values is finite where their sum may not be.  0 for a row
+// that sees no key; a row whose logits are all -inf is 0 / 0, a NaN.
 // `qrow` is 128 floats of shared memory of this warp.
 template <typename T>
 __device__ void window_row(const WinParams& p, int64_t b, int64_t h, int64_t i, float* qrow, int lane) {
@@ -139,24 +141,29 @@ __device__ void window_row(const WinParams& p, int64_t b, int64_t h, int64_t i, 
             float sum = w;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            den = __fmaf_rn(den, alpha, sum);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = __fmul_rn(acc[e], alpha);
+            const float total = __fmaf_rn(den, alpha, sum);
+            const float inv = total == 0.0f ? 0.0f : __frcp_rn(total);
+            const float keep = __fmul_rn(__fmul_rn(den, alpha), inv), share = __fmul_rn(w, inv);
+            float some[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             for (int j = 0; j < n; ++j) {
-                const float wj = __shfl_sync(0xffffffffu, w, j);
+                const float wj = __shfl_sync(0xffffffffu, share, j);
                 const T* row = v + (int64_t)(base + j) * p.vs[2];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (lane + 32 * e < p.d) acc[e] = __fmaf_rn(wj, F16<T>::to(row[lane + 32 * e]), acc[e]);
+                    if (lane + 32 * e < p.d) some[e] = __fmaf_rn(wj, F16<T>::to(row[lane + 32 * e]), some[e]);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = __fmaf_rn(acc[e], keep, some[e]);
+            den = total;
             m = m_new;
         }
     }
     const bool sees = s.sink > 0 || s.hi > s.lo;
+    const float one = __fdiv_rn(den, den);                        // NaN where no logit was above -inf
     T* out = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + i * p.os[2];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (lane + 32 * e < p.d) out[lane + 32 * e] = F16<T>::one(sees ? acc[e] / den : 0.0f);
+        if (lane + 32 * e < p.d) out[lane + 32 * e] = F16<T>::one(sees ? __fmul_rn(acc[e], one) : 0.0f);
 }
 
 constexpr int kKT = 128;                           // keys per tile
