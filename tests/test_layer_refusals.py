@@ -260,3 +260,14 @@ def test_an_output_may_be_one_argument_only(on_cpu):
     row = _t(1, 1, 1, 16)
     with pytest.raises(ValueError, match="share memory"):
         qk_norm_rope(row, _t(1, 1, 1, 16), row[0, 0, 0], out=(row, _t(1, 1, 1, 16)))
+
+
+def test_window_bounds_are_wider_than_any_position(on_cpu):
+    """The widest bounds are passed on as ones that no position reaches, inside
+    what the C entry takes."""
+    from vc_attention_b200 import window
+    q, far = _t(1, 1, 7, 16), 2 ** 39 - 1
+    for offset in (far, -far):
+        plan = window._window_plan(q, q, q, (2 ** 70, 2 ** 45), 2 ** 50, False, offset, None, None, None, None)
+        for bound in (plan.args.left, plan.args.right, plan.args.sinks):
+            assert far + 2 ** 31 < bound < 1 << 40

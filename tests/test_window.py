@@ -397,3 +397,16 @@ def test_window_sums_of_the_largest_values_stay_finite(sq, sk, d):
         assert got.isfinite().all()
         assert ((got.double() - ref).abs() <= err + eps / 2 * (ref.abs() + err)).all()
         assert (got[:, 1][seen.any(-1)] == most).all()
+
+
+@pytest.mark.parametrize("sq", [3, 200])
+def test_window_bounds_past_the_farthest_position(sq):
+    """A bound wider than any position sees every key on its side."""
+    from vc_attention_b200 import window_attention
+    g = _gen(31)
+    q, k, v = _randn((1, 1, sq, 64), BF16, g), _randn((1, 1, 50, 64), BF16, g), _randn((1, 1, 50, 64), BF16, g)
+    want = window_attention(q, k, v)
+    far = 2 ** 39 - 1
+    assert torch.equal(window_attention(q, k, v, window=(2 ** 41, 0), q_offset=far), want)
+    assert torch.equal(window_attention(q, k, v, window=(0, 2 ** 41), q_offset=-far), want)
+    assert torch.equal(window_attention(q, k, v, window=(0, 0), sinks=2 ** 41, q_offset=far), want)

@@ -20,7 +20,7 @@ def _bound(value, name):
         return -1
     if isinstance(value, bool) or not isinstance(value, int) or value < 0:
         raise ValueError(f"{name} must be a non-negative integer or None")
-    return min(value, 1 << 39)
+    return min(value, (1 << 40) - 1)           # positions stay below 2^39 + 2^31: no bound at all
 
 
 def window_attention(q, k, v, *, window=(None, None), sinks=0, causal=False, q_offset=None, kv_lens=None, scale=None,
