@@ -271,3 +271,15 @@ def test_window_bounds_are_wider_than_any_position(on_cpu):
         plan = window._window_plan(q, q, q, (2 ** 70, 2 ** 45), 2 ** 50, False, offset, None, None, None, None)
         for bound in (plan.args.left, plan.args.right, plan.args.sinks):
             assert far + 2 ** 31 < bound < 1 << 40
+
+
+def test_products_too_large_to_be_cut_are_not():
+    """73 row tiles of 2^25 chunks: more units of a cut than its 32-bit counters
+    hold, so the tiles are walked whole and need no scratch."""
+    lib = _abi.load()
+    k = 2 ** 31 - 512
+    a = _abi.LinearArgs(x=256, w=256, y=256, dtype=2, batch=73, tokens=17, n=32, heads_in=1, k_head=k, x_stride_b=16,
+                        x_stride_h=8, x_stride_s=8, w_stride=k, n_head=32)
+    assert lib.vcb_linear_workspace(ctypes.byref(a)) == 0
+    a.k_head = a.w_stride = 2 ** 24
+    assert lib.vcb_linear_workspace(ctypes.byref(a)) > 0      # the same tiles, cut

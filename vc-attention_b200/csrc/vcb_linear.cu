@@ -894,7 +894,8 @@ LinPlan plan(const vcb_linear_args* a) {
         int64_t each = (rem * q.k_chunks + pairs - 1) / pairs;
         if (each < 4) each = 4;
         const double cut = (double)(tiles / pairs) * tile + (double)each * chunk + 28 * bn + 24000;
-        const bool use_cut = rem && each < q.k_chunks && cut < whole;
+        // (the kernels count a cut's chunks in 32 bits)
+        const bool use_cut = rem && each < q.k_chunks && cut < whole && rem * q.k_chunks + each < (1ll << 31);
         const double cost = use_cut ? cut : whole;
         if (best > 0 && cost >= best) continue;
         best = cost;
