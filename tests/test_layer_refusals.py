@@ -283,3 +283,38 @@ def test_products_too_large_to_be_cut_are_not():
     assert lib.vcb_linear_workspace(ctypes.byref(a)) == 0
     a.k_head = a.w_stride = 2 ** 24
     assert lib.vcb_linear_workspace(ctypes.byref(a)) > 0      # the same tiles, cut
+
+
+def test_outputs_written_in_place_are_known_to_autograd(on_cpu):
+    """A tensor that a graph has saved may not change unnoticed, and one that
+    requires a gradient is no output, as for torch's own out= functions."""
+    x, w = _t(2, 3, 8), _t(8, 8)
+    q, k = _t(2, 4, 6, 16), _t(2, 4, 6, 16)
+    outs = [_t(2, 3, 8), _t(2, 4, 6, 16), _t(2, 4, 6, 16), _t(2, 4, 6, 16)]
+
+    def write():
+        linear(x, w, out=outs[0])
+        qk_norm_rope(q, k, out=(outs[1], outs[2]))
+        window_attention(q, k, q, out=outs[3])
+
+    leaf = torch.ones(1, requires_grad=True)
+    losses = [(leaf * o).sum() for o in outs]
+    write()
+    for loss in losses:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        outs = [torch.empty_like(o) for o in outs]
+        write()
+    write()                                     # inference tensors have no version to count
+    turned = torch.zeros((3, 2, 8), dtype=BF16).transpose(0, 1)
+    before = turned._version                    # x without rows: copied, and written once
+    linear(_t(2, 8, 3).transpose(1, 2), w, out=turned)
+    assert turned._version == before + 1
+    outs = [torch.zeros_like(o).requires_grad_() for o in outs]
+    for call in (lambda: linear(x, w, out=outs[0]), lambda: qk_norm_rope(q, k, out=(_t(2, 4, 6, 16), outs[2])),
+                 lambda: window_attention(q, k, q, out=outs[3])):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call()
+        with torch.no_grad():
+            call()

@@ -147,6 +147,8 @@ def _check_out(out, shape, like, what, inputs, may_be=None):
         raise ValueError(f"{what} must be a {tuple(shape)} tensor of the inputs' dtype and device")
     if out.shape[-1] != 1 and out.stride(-1) != 1:
         raise ValueError(f"{what} must have a contiguous last axis")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient, and results carry none")
     if _overlaps_itself(out):
         raise ValueError(f"{what} must not overlap itself")
     if may_be is not None and not _same_view(out, may_be):
@@ -154,6 +156,14 @@ def _check_out(out, shape, like, what, inputs, may_be=None):
     for t in inputs:
         if t is not None and _shares_memory(out, t):
             raise ValueError(f"{what} must not share memory with an input")
+
+
+def _written(*outs):
+    """The library writes by address: autograd has to hear of it, so that a graph
+    that saved the tensor does not read the new values in its backward pass."""
+    for out in outs:
+        if not out.is_inference():
+            torch.autograd.graph.increment_version(out)
 
 
 def _check_status(status, device):
@@ -186,7 +196,7 @@ def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, h
     Returns [B, S, N] (or [S, N]), or with ``heads_out=H`` the attention's
     input layout [B, H, S, N / H], without gate or residual.  ``out`` may be
     given, with any strides but a contiguous last axis; it may be ``residual``
-    itself and shares memory with no other input.
+    itself and shares memory with no other input.  It does not require a gradient.
 
     The call only queues work on the current stream, and its result carries no
     gradient.  ``status``: a caller-owned, zeroed one-element int32 CUDA tensor
@@ -207,6 +217,8 @@ def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, h
                       heads_out=heads_out, out=out, status=status)
     if out is None:
         out = x.new_empty(plan.shape)
+    else:
+        _written(out)
     plan.call(x.device, x=x.data_ptr(), w=weight.data_ptr(), y=out.data_ptr(), bias=_ptr(bias), gate=_ptr(gate),
               residual=_ptr(residual), status=_ptr(status))
     return out
@@ -327,6 +339,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, *, eps=
         ko = torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
         qo, ko = out
+        _written(qo, ko)
     plan.call(q.device, q=q.data_ptr(), k=k.data_ptr(), q_out=qo.data_ptr(), k_out=ko.data_ptr(),
               q_weight=_ptr(q_weight), k_weight=_ptr(k_weight), cos=_ptr(cos), sin=_ptr(sin))
     return qo, ko

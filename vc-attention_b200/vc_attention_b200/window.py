@@ -12,7 +12,7 @@ import torch
 
 from . import _abi
 from .layer import (_PLANS, _TYPES, _Plan, _check_out, _check_status, _meta, _no_rows, _packed_strides, _ptr, _remember,
-                    _require_b200)
+                    _require_b200, _written)
 
 
 def _bound(value, name):
@@ -55,6 +55,8 @@ def window_attention(q, k, v, *, window=(None, None), sinks=0, causal=False, q_o
                                 scale=scale, out=out, status=status)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        _written(out)
     plan.call(q.device, q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), kv_lens=_ptr(kv_lens),
               status=_ptr(status))
     return out
