@@ -405,3 +405,48 @@ def test_linear_few_rows_with_the_longest_sum():
     assert linear(x, w).item() == 63.0
     w[0, k - 1] = 0.5
     assert linear(x, w).item() == 47.0
+
+
+def test_an_expired_wait_is_raised_by_the_next_call():
+    """The self-test of the bounded waits (no fault, no hang: it gives up after
+    2 s) sets the flag that a projection's or attention's own expired wait sets."""
+    from vc_attention_b200 import layer, linear, window_attention
+    g = _gen(41)
+    x, w = _randn((1, 40, 64), BF16, g), _randn((32, 64), BF16, g)
+    q = _randn((1, 1, 40, 64), BF16, g)
+    own = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for call in (lambda **kw: linear(x, w, **kw), lambda **kw: window_attention(q, q, q, **kw)):
+        want = call()
+        src = torch.zeros(256, dtype=torch.int32, device="cuda")
+        report = torch.empty(4, dtype=torch.int32, device="cuda")
+        lib = layer._abi.load()
+        word = layer._shared_status(x.device)
+        layer._abi.check(lib, lib.vcb_wait_selftest(0, src.data_ptr(), word, report.data_ptr(), None))
+        torch.cuda.synchronize()
+        assert torch.equal(call(status=own), want) and own.item() == 0      # that caller looks after itself
+        with pytest.raises(RuntimeError, match="an earlier .* wait expired"):
+            call()
+        assert torch.equal(call(), want)
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    import pathlib
+    import subprocess
+    import sys
+    code = """
+import torch
+from vc_attention_b200 import linear, window_attention
+x = torch.ones((1, 40, 64), device="cuda", dtype=torch.bfloat16)
+w = torch.ones((32, 64), device="cuda", dtype=torch.bfloat16)
+q = torch.ones((1, 1, 40, 64), device="cuda", dtype=torch.bfloat16)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y, o = linear(x, w), window_attention(q, q, q)
+graph.replay()
+torch.cuda.synchronize()
+assert (y == 64).all() and (o == 1).all()
+print("captured")
+"""
+    run = subprocess.run([sys.executable, "-c", code], cwd=pathlib.Path(__file__).resolve().parents[1] / "vc-attention_b200",
+                         capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "captured" in run.stdout, run.stderr[-2000:]

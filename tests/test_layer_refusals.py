@@ -318,3 +318,15 @@ def test_outputs_written_in_place_are_known_to_autograd(on_cpu):
             call()
         with torch.no_grad():
             call()
+
+
+def test_flags_of_an_earlier_call_are_raised_once(monkeypatch):
+    held = torch.zeros(1, dtype=torch.int32)
+    word = ctypes.c_int32.from_address(held.data_ptr())
+    monkeypatch.setattr(layer, "_WORDS", {0: (held, word)})
+    device = torch.device("cuda", 0)
+    for flag, match in ((_abi.FLAG_TIMEOUT, "wait expired"), (_abi.FLAG_INTERNAL, "layout check")):
+        held[0] = flag
+        with pytest.raises(RuntimeError, match="an earlier linear or window_attention call on cuda:0.*" + match):
+            layer._shared_status(device)
+        assert held.item() == 0 and layer._shared_status(device) == held.data_ptr()

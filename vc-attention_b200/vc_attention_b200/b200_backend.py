@@ -158,12 +158,17 @@ def raise_for_status(status):
     flags = ctypes.c_int32(0)
     with torch.cuda.device(status.device):
         _abi.check(lib, lib.vcb_read_status(status.data_ptr(), _stream(status.device), ctypes.byref(flags)))
-    if flags.value & _abi.FLAG_NONFINITE:
+    raise_for_flags(flags.value, "b200_fp8 attention kernel")
+
+
+def raise_for_flags(flags, what):
+    """The exception for the flags of a status word, if any is set."""
+    if flags & _abi.FLAG_NONFINITE:
         raise ValueError("Q/K/V must be finite")
-    if flags.value & _abi.FLAG_TIMEOUT:
-        raise RuntimeError("b200_fp8 attention kernel: a bounded device wait expired")
-    if flags.value & _abi.FLAG_INTERNAL:
-        raise RuntimeError("b200_fp8 attention kernel: device layout check failed")
+    if flags & _abi.FLAG_TIMEOUT:
+        raise RuntimeError(f"{what}: a bounded device wait expired")
+    if flags & _abi.FLAG_INTERNAL:
+        raise RuntimeError(f"{what}: device layout check failed")
 
 
 @torch.no_grad()
@@ -277,6 +282,7 @@ def preflight(device="cuda:0"):
     """Fail loudly unless ExpCast bytes and the fused FP8 path work
     (cuda_backend.py:69-88), and the operators around it."""
     from .core import Config, attention
+    from .layer import _shared_status
 
     device = torch.device(device)
     if device.type != "cuda" or torch.cuda.get_device_capability(device) != (10, 0):
@@ -295,6 +301,7 @@ def preflight(device="cuda:0"):
         torch.testing.assert_close(actual, torch.full_like(actual, 3), rtol=2e-5, atol=2e-5)
     _preflight_layer(device)
     torch.cuda.synchronize(device)
+    _shared_status(torch.empty(0, device=device).device)
     return {"device": str(device), "name": torch.cuda.get_device_name(device), "preflight": "passed",
             **build_info()}
 

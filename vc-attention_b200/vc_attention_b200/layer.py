@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 
 import torch
 
@@ -90,6 +91,33 @@ def _remember(key, plan):
     return plan
 
 
+# Where calls without a status word of their own leave their flags: a word of
+# pinned host memory for each device, which the next such call reads without
+# waiting for the device.  A wait that gave up is a fault of the library; its call
+# has returned by then, but it does not go unnoticed.
+_WORDS = {}
+_WORDS_LOCK = threading.Lock()
+
+
+def _shared_status(device):
+    """The address of the device's shared status word.  Raises what an earlier
+    call left there, once."""
+    word = _WORDS.get(device.index)
+    if word is None:
+        with _WORDS_LOCK:
+            if device.index not in _WORDS:
+                held = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+                _WORDS[device.index] = held, ctypes.c_int32.from_address(held.data_ptr())
+            word = _WORDS[device.index]
+    held, flags = word
+    if flags.value:
+        from .b200_backend import raise_for_flags
+
+        value, flags.value = flags.value, 0
+        raise_for_flags(value, f"an earlier linear or window_attention call on {device}, whose output is incomplete")
+    return held.data_ptr()
+
+
 class _Plan:
     """Arguments without addresses (``args``), the scratch bytes for 16-byte
     aligned operands (``need``), the C entry points, and the operands that have
@@ -112,6 +140,8 @@ class _Plan:
         a = self.cls.from_buffer_copy(self.args)
         for name, value in pointers.items():
             setattr(a, name, value)
+        if pointers.get("status", 0) is None:
+            a.status = _shared_status(device)
         need = self.need
         if self.workspace is not None and any(pointers[name] & 15 for name in self.operands):
             need = self.workspace(ctypes.byref(a))
@@ -199,9 +229,11 @@ def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, h
     itself and shares memory with no other input.  It does not require a gradient.
 
     The call only queues work on the current stream, and its result carries no
-    gradient.  ``status``: a caller-owned, zeroed one-element int32 CUDA tensor
-    that receives the kernel's flags for ``b200_backend.raise_for_status`` (an
-    expired device wait)."""
+    gradient.  An expired device wait, which leaves the output incomplete, is
+    raised by the next call of this kind on the device (RuntimeError).
+    ``status`` takes that over: a caller-owned, zeroed one-element int32 CUDA
+    tensor that receives the kernel's flags for
+    ``b200_backend.raise_for_status``."""
     key = ("linear", _meta(x), _meta(weight), _meta(bias), activation, _meta(gate), _meta(residual), bool(heads_in),
            heads_out, type(heads_out), _meta(out), _meta(status))
     plan = _PLANS.get(key)
