@@ -450,3 +450,42 @@ print("captured")
     run = subprocess.run([sys.executable, "-c", code], cwd=pathlib.Path(__file__).resolve().parents[1] / "vc-attention_b200",
                          capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and "captured" in run.stdout, run.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("b,s,heads,k,n", [
+    (1, 40, 1, 20000, 96), (3, 100, 1, 24000, 72), (1, 17, 1, 17832, 8), (2, 70, 192, 24576, 200),       # cut tiles alone
+    (1, 40, 1, 20001, 95),                                                                               # off the grid
+    (1, 6273, 1, 12040, 272), (1, 9586, 1, 9504, 240),                                                   # behind whole ones
+])
+def test_linear_tiles_cut_along_k(b, s, heads, k, n, dtype):
+    """These shapes are cut (their scratch says so), and every epilogue and
+    layout runs behind the join."""
+    from vc_attention_b200 import layer, linear
+    g = _gen(k + n)
+    x, w = _randn((b, s, k), dtype, g), _randn((n, k), dtype, g, k ** -0.5)
+    plan = layer._linear_plan(x, w, None, None, None, None, False, None, None, None)
+    copies = 0 if k % 8 == 0 else 2 * (b * s + n) * (k + 7) + 512
+    assert plan.need > copies
+    res, bias, gate = _randn((b, s, n), dtype, g), _randn((n,), FP32, g), _randn((b, 1, n), FP32, g)
+    kw = dict(activation="gelu", gate=gate, residual=res)
+    want, err = _linear_ref(x, w, bias, **kw)
+    got = linear(x, w, bias, **kw)
+    _check(got, want, err)
+    assert torch.equal(linear(x, w, bias, **kw), got)
+    # in place on the residual, and inside a larger buffer on and off the 16-byte grid
+    held = res.clone()
+    assert torch.equal(linear(x, w, bias, activation="gelu", gate=gate, residual=held, out=held), got)
+    for lo in (3, 8):
+        buf = torch.full((b, s + 2, n + 16), 7.0, device="cuda", dtype=dtype)
+        out = buf[:, 1:s + 1, lo:lo + n]
+        linear(x, w, bias, out=out, **kw)
+        assert torch.equal(out, got)
+        out.fill_(7.0)
+        assert (buf == 7.0).all()
+    if heads > 1:
+        xh = x.view(b, s, heads, k // heads).transpose(1, 2).contiguous()
+        _check(linear(xh, w, bias, heads_in=True, **kw), want, err)
+    if n % 8 == 0:
+        split = linear(x, w, bias, heads_out=4)
+        _check(split.transpose(1, 2).reshape(b, s, n), *_linear_ref(x, w, bias))
