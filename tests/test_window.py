@@ -410,3 +410,67 @@ def test_window_bounds_past_the_farthest_position(sq):
     assert torch.equal(window_attention(q, k, v, window=(2 ** 41, 0), q_offset=far), want)
     assert torch.equal(window_attention(q, k, v, window=(0, 2 ** 41), q_offset=-far), want)
     assert torch.equal(window_attention(q, k, v, window=(0, 0), sinks=2 ** 41, q_offset=far), want)
+
+
+@pytest.mark.parametrize("sq,sk", [(1, 600), (200, 600), (300, 3000)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_window_non_finite_keys_give_what_the_definition_gives(sq, sk, bad):
+    """A key with one bad channel: a NaN or +inf logit makes its rows NaN, a
+    -inf logit takes the key out of them; rows that do not see it keep their value."""
+    g = _gen(sq + 5)
+    q, k, v = _randn((1, 2, sq, 128), BF16, g), _randn((1, 2, sk, 128), BF16, g), _randn((1, 2, sk, 128), BF16, g)
+    kw = dict(window=(60, 0), sinks=2, causal=True)
+    _, (clean, clean_err), seen = _run(q, k, v, **kw)
+    for key in (sk - 30, sk - 100, 1, sk - 1):
+        held = k[0, 1, key].clone()
+        k[0, 1, key, 3] = bad
+        got, _, _ = _run(q, k, v, **kw)
+        k[0, 1, key] = held
+        sees = seen[0, :, key]
+        _check(got[:, :, ~sees], clean[:, :, ~sees], clean_err[:, :, ~sees])
+        _check(got[:, :1], clean[:, :1], clean_err[:, :1])
+        sign = q[0, 1, :, 3].sign() * bad                     # the logit's infinity, or NaN
+        gone = sees & (sign < 0)
+        assert got[0, 1][sees & ~gone].isnan().all()
+        without = seen.clone()
+        without[:, :, key] = False
+        ref, err = _reference(q, k, v, without, 128 ** -0.5)
+        _check(got[:, 1:, gone], ref[:, 1:, gone], err[:, 1:, gone])
+
+
+@pytest.mark.parametrize("b,h,sq,sk,d", [
+    (2, 41, 300, 1500, 128), (2, 41, 300, 1500, 80), (2, 41, 300, 1500, 41), (2, 41, 300, 1500, 64),     # two query tiles
+    (2, 151, 3, 3000, 128), (2, 151, 3, 3000, 72),                                                       # one
+])
+@pytest.mark.parametrize("mask", [0, 3, 4])
+def test_window_whole_items_and_items_cut_along_their_keys(b, h, sq, sk, d, mask):
+    """More items than CTAs at once: those behind the full rounds are cut along
+    their keys.  Entries of different lengths, padding and a key that hold NaN."""
+    from vc_attention_b200 import window
+    g = _gen(sq + d + mask)
+    q, k, v = _randn((b, h, sq, d), BF16, g), _randn((b, h, sk, d), BF16, g), _randn((b, h, sk, d), BF16, g)
+    kw = dict(dict(causal=mask == 3, window=(None, None), sinks=0), **MASKS[mask])
+    if mask:
+        kw["window"] = tuple(None if x is None else 16 * x for x in kw["window"])
+    slots = torch.cuda.get_device_properties(0).multi_processor_count * (2 if sq <= 128 else 1)
+    assert b * h * -(-sq // (128 if sq <= 128 else 256)) > slots
+    if d % 8 == 0:                          # nothing is copied, so scratch means items cut along their keys
+        plan = window._window_plan(q, k, v, kw["window"], kw["sinks"], kw["causal"], None, None, None, None, None)
+        assert plan.need > 0
+    lens = [sk, sk - 389]
+    clean, (ref, err), seen = _run(q, k, v, lens=lens, **kw)
+    _check(clean, ref, err)
+    for e, n in enumerate(lens):
+        k[e, :, n:], v[e, :, n:] = float("nan"), float("inf")
+    assert torch.equal(_run(q, k, v, lens=lens, **kw)[0], clean)
+    for e, head in ((0, 0), (b - 1, h - 1)):                  # the first item and the last
+        key = lens[e] - 300
+        held = v[e, head, key].clone()
+        v[e, head, key] = float("nan")
+        got, _, _ = _run(q, k, v, lens=lens, **kw)
+        v[e, head, key] = held
+        sees = seen[e, :, key]
+        assert got[e, head][sees].isnan().all()
+        _check(got[e, head][~sees], ref[e, head][~sees], err[e, head][~sees])
+        got[e, head] = clean[e, head]
+        assert torch.equal(got, clean)
