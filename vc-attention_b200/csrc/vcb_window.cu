@@ -142,7 +142,10 @@ __device__ void window_row(const WinParams& p, int64_t b, int64_t h, int64_t i, 
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             const float total = __fmaf_rn(den, alpha, sum);
-            const float inv = total == 0.0f ? 0.0f : __frcp_rn(total);
+            // (a correctly rounded reciprocal spilled two registers of the softmax warps;
+            // one Newton step takes the approximate one, of 1 or more, to half a step)
+            float inv = total == 0.0f ? 0.0f : __fdividef(1.0f, total);
+            inv = __fmaf_rn(__fmaf_rn(-total, inv, 1.0f), inv, inv);
             const float keep = __fmul_rn(__fmul_rn(den, alpha), inv), share = __fmul_rn(w, inv);
             float some[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             for (int j = 0; j < n; ++j) {
