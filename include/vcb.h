@@ -262,7 +262,7 @@ typedef struct {
     const void* gate;               /* or NULL; strides of 0 broadcast */
     int gate_dtype;                 /* vcb_dtype */
     int64_t gate_stride_b, gate_stride_s;
-    const void* residual;           /* or NULL; may be y itself */
+    const void* residual;           /* or NULL; may be y itself, which shares memory with no other operand */
     int64_t residual_stride_b, residual_stride_s;
     void* y;
     int64_t n_head;                 /* divides n */
@@ -279,8 +279,8 @@ VCB_API int vcb_linear(const vcb_linear_args* args, void* stream);
 /* Per head row x of Q and of K: n = x * weight / sqrt(mean(x^2) + eps) (norm;
  * else n = x * weight), then (a, b) -> (a cos - b sin, a sin + b cos) for the
  * rotary / 2 pairs: channels (2i, 2i + 1) when interleaved, (i, i + rotary / 2)
- * otherwise.  Tokens at or behind `rows` are not rotated.  An output may be
- * its own input. */
+ * otherwise.  Tokens at or behind `rows` are not rotated.  q_out may be q and
+ * k_out k; neither shares memory with another operand. */
 typedef struct {
     const void* q; const void* k;
     void* q_out; void* k_out;

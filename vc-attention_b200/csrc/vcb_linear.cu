@@ -278,7 +278,7 @@ __device__ void lin_mma(const LinParams& p, uint8_t* smem, const LinBars& B, con
 // 0.5 y (1 + erf(y / sqrt 2)) without the cancellation for y < 0: with
 // z = |y| / sqrt 2 and t = 1 / (1 + 0.45 z), erfc(z) = t q(t) exp(-z^2), q a degree-7
 // fit to erfc(z) exp(z^2) / t over z in [0, 60] (least squares reweighted towards
-// the largest relative error, which is 6e-7).  No branches.
+// the largest relative error, which is 6.7e-7).  No branches.
 __device__ __forceinline__ float gelu_erf(float y) {
     const float z = 0.70710678118654752f * fabsf(y);
     const float t = __fdividef(1.0f, __fmaf_rn(0.45f, z, 1.0f));
@@ -880,9 +880,13 @@ LinPlan plan(const vcb_linear_args* a) {
     // cut along K.  Cost in clocks, fitted to timelines of one pair: a 64-channel
     // chunk takes the longer of its products (2.2 a column) and its loads (100
     // bytes a clock); the last epilogue 25 a column; a cut writes its sums (28 a
-    // column) and is joined by a second launch (24000).  A width that fills the
-    // last round is mostly better than a cut: 256 x 5120 x 5120 BF16 takes 24.6 us
-    // cut at 256 columns, 16.0 whole at 96.
+    // column) and is joined by a second launch (24000).  It leaves out the launch,
+    // the first loads and the clocks under load, so it ranks widths and is below
+    // the time of a call: for K = N = 5120 at 1.9 GHz 11.0 us of 15.6 at 64 rows,
+    // 17.8 of 23.2 at 512, 32.2 of 45.9 at 1024.  A width that fills the last round
+    // is mostly better than a cut: 256 x 5120 x 5120 BF16 takes 24.6 us cut at 256
+    // columns, 16.0 whole at 96.  Long sums over few tiles are cut (40 x 20000 x 96),
+    // and a few tiles behind a full round (6273 x 12040 x 272).
     const int64_t pairs = sm_count() / 2;
     const int64_t tile_rows = q.rows < 128 ? q.rows : 128;
     double best = 0;

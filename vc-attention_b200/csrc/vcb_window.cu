@@ -13,8 +13,8 @@
 // Work decomposition.  A CTA owns NQ (1 or 2) tiles of 128 queries of one
 // head; items that would not fill the last round of CTAs are cut along their
 // keys, and window_join_kernel joins the parts in a fixed order.  Per key tile and query
-// tile: S = Q K^T into tensor memory (tcgen05, 128 x 128), the softmax
-// warpgroup of the query tile (one thread per row) turns S into P = 2^(s - m)
+// tile: S = Q K^T into tensor memory (tcgen05, 128 x 128), the query tile's
+// eight softmax warps (two lanes per row, 64 keys each) turn S into P = 2^(s - m)
 // in 16 bits over S's own columns, and O += P V adds onto the row's sums in
 // tensor memory.  V stays [key][channel] as it comes: it is the N-major B
 // operand.  With two query tiles one tile's products run under the other's
@@ -50,10 +50,10 @@
 // window_row, which reads only the keys that the row sees.  Finite values near
 // the end of BF16's range take that way too: P V sums them before the division.
 //
-// Roles (128 + 128 NQ threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2
-// clears V rows behind the last key, warp 3 tensor memory; then one softmax
-// warpgroup per query tile, which also writes the output.  Every mbarrier wait
-// is bounded; a CTA that gives up drains and frees its tensor memory.
+// Roles (128 + 256 NQ threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2
+// clears V rows behind the last key, warp 3 tensor memory; then eight softmax
+// warps (two warpgroups) per query tile, which also write the output.  Every
+// mbarrier wait is bounded; a CTA that gives up drains and frees its tensor memory.
 #include "vcb_f16.cuh"
 
 namespace vcb {
@@ -187,7 +187,8 @@ template <int HD, int NQ> struct WinTile {
     static constexpr uint32_t kCols = NQ == 2 ? 512 : 256;
     static constexpr uint32_t kColO = NQ * 128;
     // setmaxnreg shares: control warps, softmax warps (64 / 104 with two query
-    // tiles: 5.23 ms against 5.15; 64 / 88 with one spills)
+    // tiles: 5.23 ms against 5.15).  With one tile, two CTAs per SM leave 80 a thread
+    // at launch: 20 bytes spill, 368 with 64 / 88.
     static constexpr int kRegsCtl = 32, kRegsSoft = NQ == 2 ? 112 : 104;
     static constexpr int kRegSplit = 128 * kRegsCtl + 256 * NQ * kRegsSoft;
     static_assert(kSmem <= 232448 / kCtas - (kCtas - 1) * 1024, "shared memory of one CTA");
@@ -444,7 +445,7 @@ __device__ void win_mma(const WinItem& it, uint8_t* smem, const WinBars& B, uint
     drain_wait(B.drain, 0);
 }
 
-// Bits [a, b) of the 32-key word that starts at key 32 w of a tile.
+// The lowest x bits (none for x <= 0, all for x >= 32).
 __device__ __forceinline__ uint32_t bits_below(int x) { return x <= 0 ? 0u : x >= 32 ? 0xffffffffu : (1u << x) - 1u; }
 
 // Warp (quarter, sub) of query tile w owns rows 32 quarter + 16 sub + [0, 16);
@@ -779,8 +780,7 @@ WinPlan plan(const vcb_window_args* a) {
     // Key tiles of a query tile (an upper bound where lengths are on the device).
     auto tiles = [](int64_t n) { return (n + kKT - 1) / kKT; };
     const int64_t all = tiles(a->sk);
-    int64_t right = a->causal ? 0 : a->right;
-    if (a->causal && a->right >= 0 && a->right < right) right = a->right;
+    const int64_t right = a->causal ? 0 : a->right;
     int64_t t = all;
     if (a->left >= 0 && right >= 0) {
         const int64_t span = tiles(a->left + right + (a->sq < rows ? a->sq : rows)) + 1;
