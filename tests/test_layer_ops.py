@@ -489,3 +489,18 @@ def test_linear_tiles_cut_along_k(b, s, heads, k, n, dtype):
     if n % 8 == 0:
         split = linear(x, w, bias, heads_out=4)
         _check(split.transpose(1, 2).reshape(b, s, n), *_linear_ref(x, w, bias))
+
+
+def test_calls_under_a_default_device(monkeypatch):
+    from vc_attention_b200 import layer, linear, window_attention
+    g = _gen(43)
+    x, w = _randn((1, 40, 64), BF16, g), _randn((32, 64), BF16, g)
+    q = _randn((1, 1, 40, 64), BF16, g)
+    want = linear(x, w), window_attention(q, q, q)
+    torch.cuda.synchronize()
+    held = layer._WORDS
+    monkeypatch.setattr(layer, "_WORDS", {})
+    with torch.device("cuda"):
+        got = linear(x, w), window_attention(q, q, q)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and layer._WORDS.keys() == held.keys()

@@ -106,7 +106,7 @@ def _shared_status(device):
     if word is None:
         with _WORDS_LOCK:
             if device.index not in _WORDS:
-                held = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+                held = torch.zeros(1, dtype=torch.int32, device="cpu", pin_memory=True)
                 _WORDS[device.index] = held, ctypes.c_int32.from_address(held.data_ptr())
             word = _WORDS[device.index]
     held, flags = word
@@ -345,8 +345,9 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, *, eps=
 
     Returns (q, k) as contiguous BNSD tensors, or writes ``out=(q_out,
     k_out)``, for example rows of a K buffer; q_out may be ``q`` itself and
-    k_out ``k``, and neither shares memory with another argument.  The call only queues work on the current stream, and its results
-    carry no gradient."""
+    k_out ``k``, and neither shares memory with another argument.  The call
+    only queues work on the current stream, and its results carry no
+    gradient."""
     if out is None:
         outs = None
     else:
