@@ -142,8 +142,9 @@ __device__ void window_row(const WinParams& p, int64_t b, int64_t h, int64_t i, 
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             const float total = __fmaf_rn(den, alpha, sum);
-            // (a correctly rounded reciprocal spilled two registers of the softmax warps;
-            // one Newton step takes the approximate one, of 1 or more, to half a step)
+            // (a correctly rounded reciprocal here spilled two registers of the softmax warps,
+            // as did an early end at a row of NaNs: 6 % of the whole kernel's time.  One Newton
+            // step takes the approximate one to about half a step)
             float inv = total == 0.0f ? 0.0f : __fdividef(1.0f, total);
             inv = __fmaf_rn(__fmaf_rn(-total, inv, 1.0f), inv, inv);
             const float keep = __fmul_rn(__fmul_rn(den, alpha), inv), share = __fmul_rn(w, inv);
